@@ -85,6 +85,9 @@ int tg_ctx_selftest_wait(tg_ctx *ctx, uint64_t limit_ns);
 /* ---- Memory (Context::memory_in / buffer_in, crates/vulkan/src/context.rs:487-495) -------- */
 
 int tg_mem_alloc(tg_ctx *ctx, uint64_t bytes, tg_residence residence, tg_mem **out);
+/* A buffer over device memory the caller owns (of the context's device; it has to outlive the buffer
+ * and what uses it): bindings and copies take it as any other, tg_mem_free leaves the memory. */
+int tg_mem_wrap(tg_ctx *ctx, void *device_ptr, uint64_t bytes, tg_mem **out);
 int tg_mem_free(tg_mem *mem);
 uint64_t tg_mem_size(const tg_mem *mem);
 /* The buffer's address for the GPU (a device pointer, or the mapped address of pinned memory). */
@@ -205,7 +208,66 @@ typedef enum {
      * x f32 [rows][feat][frames] (read and written): x -= dt times the guided velocity of tokens
      * first .. first + frames - 1                                                dit_euler.comp */
     TG_KERNEL_DIT_EULER = 26,
-    TG_KERNEL_COUNT = 27
+    /* ---- A paged, prefix-sharing batch (no counterpart in tgtts-v4) ------------------------------
+     * A cache of pages is a slot cache whose slots are the pages: k and v T [slots pages][kv_heads]
+     * [capacity positions of a page][hd], capacity a multiple of 16, slots x capacity below 2^32 - 1.
+     * A request's first `first` positions are the batch's shared prefix, kept once in the pages
+     * `shared` lists; the positions from `first` on are its own, in the pages of its row of `table`
+     * (its own positions i in page i / capacity of it). Of these four kernels' bindings no output
+     * may overlap another binding, but for LOGITS_PICK's out, which may be its logits.
+     *
+     * held u32 [seqs], fresh u32 [seqs], free u32 [n], table u32 [seqs][stride] (read and written)
+     * -> table, at u32 [2 rows], place u32 [rows], starts u32 [seqs + 1], next u32 [seqs],
+     * counts u32 [4]: request s holds held[s] own positions and runs fresh[s] more this step. Its
+     * new pages are the next ones of `free`, in request order; table entries of pages it holds, and
+     * those past its last page, are left. Requests are served in order up to the first that does
+     * not fit (too few free pages, rows, or table entries, or positions past 2^32 - 2), and that one
+     * and the ones behind it not at all. Served requests' rows are packed in order: row starts[s] + i
+     * is at position first + held[s] + i of request s (`at`, as tg_batch_placement's words), stored
+     * at place = page x capacity + offset; rows behind the last are spare (TG_SPARE in `at` and
+     * `place`). next: held + fresh of a served request, held of another. counts: the pages taken, the
+     * rows placed, the requests served, and the pages that all would have taken (TG_SPARE when
+     * more). A page past the cache gives place TG_SPARE and the kernel error word. seqs at most
+     * 16384; n may be 0 (free then any 16 bytes). dtype is not used. */
+    TG_KERNEL_PAGE_PLAN = 27,
+    /* at u32 [2 rows], place u32 [rows], c f32 (T when params.flags bit 1) [rows][(heads + 2 kv) hd],
+     * cos f32, sin f32 [n][k / 2] -> q T [rows][heads][hd], k pages T, v pages T: ROPE_ROWS over
+     * places of pages, the first k (even, at most hd) dimensions of each head rotated as pairs
+     * (i, i + k / 2), or (2 i, 2 i + 1) with params.flags bit 0, the others as they are; all as they
+     * are when params.rope is 0 (k 0, cos and sin any 16 bytes). A row whose position is TG_SPARE
+     * writes nothing; one whose place is TG_SPARE writes q alone. A position of n or more, or a
+     * place past the cache, is skipped with the kernel error word. Of rows with the same place one,
+     * not said which, is kept. */
+    TG_KERNEL_ROPE_PAGES = 28,
+    /* q T [rows][heads][hd], k pages T, v pages T, at u32 [2 rows] (a position of at least `first`,
+     * then a request), table u32 [seqs][stride], shared u32 [ceil(first / capacity)] (any 16 bytes
+     * when first is 0), work (its size by tg_dispatch_needs; its
+     * contents free between dispatches, so dispatches in one stream may share it)
+     * -> out T [rows][heads][hd]: each row attends to the shared prefix and to its request's own
+     * positions up to its own, softmax(q k / sqrt(hd)) v. The prefix is read once for many rows.
+     * Rows may belong to one request (several new positions, each seeing those before it). A spare
+     * row's output is left. A position below `first` or past the table, a request of seqs or more,
+     * or a page past the cache is reported by the kernel error word (the row's output is left, or
+     * for a page meaningless). A row's result is the same bits whatever rows run beside it, for one
+     * shared prefix. At most 65535 rows. */
+    TG_KERNEL_ATTENTION_PAGES = 29,
+    /* logits T [rows][stride], seen u32 [k], spans u32 [rows][6], penalties f32 [rows][3], bias_ids
+     * u32 [k1], bias f32 [k1], masks u32 [m][ceil(n / 32)] -> out T [rows][stride], pick u32 [rows]:
+     * controls on logits over a vocabulary of n tokens, and the greedy choice. A row's span: where
+     * its history starts in `seen`, its prompt tokens, its generated tokens behind them, where its
+     * biases start, their number, and its mask (TG_SPARE: none). Its penalties: repetition r,
+     * presence, frequency. With c a token's generated occurrences, x its logit:
+     *   x = x / r if x > 0 else x r   (tokens that occur in the history at all)
+     *   x = x - c frequency - (c > 0) presence
+     *   x = x + bias                  (of a token listed twice the last entry)
+     *   x = -inf                      where the mask's bit (bit t % 32 of word t / 32) is 0
+     * in f32, stored in T; the columns from n to stride are left. pick: the lowest token of the
+     * largest stored value above -inf (never a NaN), TG_SPARE when there is none. Tokens past the
+     * vocabulary in seen or bias_ids count for nothing. A span past its array, or a mask of m or
+     * more, leaves the row's out and pick as they were, with the kernel error word. k, k1 and m may
+     * be 0 (the arrays then any 16 bytes). Histories of at most 2^31 - 1 tokens. */
+    TG_KERNEL_LOGITS_PICK = 30,
+    TG_KERNEL_COUNT = 31
 } tg_kernel_id;
 
 /* The stack's shape, as one struct all kernels' params share (decode.rs:66-83 `Shape`, plus the
@@ -249,6 +311,16 @@ typedef struct {
 /* Context::dispatch (crates/vulkan/src/context.rs:520): runs one dispatch, waits, and gives its
  * GPU time in ns (may be NULL). */
 int tg_dispatch_once(tg_ctx *ctx, const tg_dispatch *d, double *ns);
+/* The same dispatch, with the same checks, enqueued on a stream of the caller's (a cudaStream_t of the
+ * context's device; NULL: the legacy stream; TG_ECUDA for another device's) without waiting; it allocates nothing, so it may be
+ * captured into the caller's CUDA graph. The buffers have to live until the work is done, and
+ * what the kernels report in the context's error word comes with the next tg_ctx_synchronize after
+ * that. */
+int tg_dispatch_enqueue(tg_ctx *ctx, const tg_dispatch *d, void *stream);
+/* What a dispatch's checks ask of its bindings, without a device: the bytes each binding of `kernel`
+ * must hold for these params, in order, into `bytes` (room for n; may be NULL when n is 0), their number
+ * into *count. Refuses what tg_dispatch_once refuses of the params (TG_EINVAL, TG_ESHAPE). */
+int tg_dispatch_needs(uint32_t kernel, const tg_params *p, uint64_t *bytes, size_t n, size_t *count);
 
 /* ---- Programs (Context::record / Recording, crates/vulkan/src/recording.rs:161-260, :599-760).
  * A program is a chain of dispatches, checked once and captured into one CUDA graph, run as

@@ -98,6 +98,7 @@ KERNELS = {
     "gemm_silu": 14, "attention_rows_tc": 15, "gemm_qkv_rope": 16, "gemv_linear": 17,
     "local_norm": 18, "local_partial": 19, "local_gate_up": 20, "local_attention": 21,
     "local_add_norm": 22, "local_rows": 23, "local_embed": 24, "cfm_noise": 25, "dit_euler": 26,
+    "page_plan": 27, "rope_pages": 28, "attention_pages": 29, "logits_pick": 30,
 }
 
 
@@ -163,6 +164,7 @@ SIGNATURES = {
     "tg_ctx_stream": (_P, [_P]),
     "tg_ctx_selftest_wait": (_I, [_P, _U64]),
     "tg_mem_alloc": (_I, [_P, _U64, _I, ctypes.POINTER(_P)]),
+    "tg_mem_wrap": (_I, [_P, _P, _U64, ctypes.POINTER(_P)]),
     "tg_mem_free": (_I, [_P]),
     "tg_mem_size": (_U64, [_P]),
     "tg_mem_device_ptr": (_P, [_P]),
@@ -171,6 +173,8 @@ SIGNATURES = {
     "tg_mem_fill": (_I, [_P, _U64, _U32, _U64]),
     "tg_copy_regions": (_I, [_P, _P, _P, ctypes.POINTER(TgRegion), _SZ]),
     "tg_dispatch_once": (_I, [_P, ctypes.POINTER(TgDispatch), _DP]),
+    "tg_dispatch_enqueue": (_I, [_P, _P, _P]),
+    "tg_dispatch_needs": (_I, [_U32, ctypes.POINTER(TgParams), ctypes.POINTER(_U64), _SZ, ctypes.POINTER(_SZ)]),
     "tg_program_create": (_I, [_P, ctypes.POINTER(TgDispatch), _SZ, _I, ctypes.POINTER(_P)]),
     "tg_program_destroy": (_I, [_P]),
     "tg_program_start": (_I, [_P]),
@@ -498,6 +502,19 @@ class Memory:
         self.handle = h
         self.nbytes = nbytes
 
+    @classmethod
+    def wrap(cls, ctx: Context, tensor) -> "Memory":
+        """A buffer over a contiguous CUDA tensor of the context's device (anything with `data_ptr()`,
+        `nbytes` and `is_contiguous()`), which it keeps alive; nothing is copied."""
+        if not tensor.is_contiguous():
+            raise ShapeError("a tensor that is not contiguous")
+        self = cls.__new__(cls)
+        self.ctx, self.handle, self.nbytes, self._tensor = ctx, None, tensor.nbytes, tensor
+        h = ctypes.c_void_p()
+        check(library().tg_mem_wrap(ctx.handle, ctypes.c_void_p(tensor.data_ptr()), tensor.nbytes, ctypes.byref(h)))
+        self.handle = h
+        return self
+
     @property
     def device_ptr(self) -> int:
         return int(library().tg_mem_device_ptr(self.handle) or 0)
@@ -546,6 +563,49 @@ def dispatch_once(ctx: Context, kernel: str, p: TgParams,
     ns = ctypes.c_double()
     check(library().tg_dispatch_once(ctx.handle, ctypes.byref(d), ctypes.byref(ns)))
     return ns.value
+
+
+class Dispatch:
+    """One kernel-table dispatch, made once and enqueued as often as needed, on any stream of the
+    context's device, without waiting (tg_dispatch_enqueue; inside a CUDA graph capture too).
+    `bindings` are buffers (the whole of each) or (buffer, offset, bytes). `params` may be changed
+    between calls: each is checked against the bindings' sizes."""
+
+    def __init__(self, ctx: Context, kernel: str, p: TgParams, bindings, label: str = ""):
+        if kernel not in KERNELS:
+            raise InvalidError(f"no kernel {kernel!r}")
+        parts = [b if isinstance(b, tuple) else (b, 0, b.nbytes) for b in bindings]
+        self.ctx, self.kernel, self.params = ctx, kernel, p
+        self._keep = ([m for m, _, _ in parts], label.encode() or None,
+                      (TgBinding * len(parts))(*[TgBinding(m.handle, o, n) for m, o, n in parts]))
+        self._c = TgDispatch(KERNELS[kernel], ctypes.pointer(p), self._keep[2], len(parts), self._keep[1])
+        self._at = ctypes.addressof(self._c)
+        self._enqueue = library().tg_dispatch_enqueue
+
+    def enqueue(self, stream: int = 0) -> None:
+        """Runs it on `stream` (a cudaStream_t as an integer, 0 the legacy stream; `ctx.stream` the
+        context's own), in that stream's order."""
+        for m in self._keep[0]:
+            if not m.handle:
+                raise InvalidError(f"{self.kernel}: a buffer that was freed")
+        status = self._enqueue(self.ctx.handle, self._at, stream)
+        if status:
+            check(status)
+
+
+def needs(kernel: str, p: TgParams) -> list[int]:
+    """The bytes each binding of a kernel-table dispatch must hold for these params, in order; raises
+    for params the kernel does not take. Needs no GPU."""
+    if kernel not in KERNELS:
+        raise InvalidError(f"no kernel {kernel!r}")
+    room, count = (ctypes.c_uint64 * 64)(), ctypes.c_size_t()
+    check(library().tg_dispatch_needs(KERNELS[kernel], ctypes.byref(p), room, 64, ctypes.byref(count)))
+    return list(room[:count.value])
+
+
+def attention_pages_work(p: TgParams) -> int:
+    """The bytes of attention_pages's work binding for these params."""
+    return needs("attention_pages", p)[6]
 
 
 class Program:

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <algorithm>
 #include <cstring>
+#include <new>
 #include <thread>
 
 #include "tg_common.cuh"
@@ -68,6 +69,7 @@ static bool is_local(uint32_t k) { return k >= TG_KERNEL_LOCAL_NORM && k <= TG_K
 struct Need {
     const char *name;
     uint64_t bytes;
+    bool empty = false;  // nothing is read of it: any 16 bytes do
 };
 
 // What each binding of a dispatch must hold, in order (the kernels index by their params and do
@@ -82,6 +84,7 @@ static int needs(const Launch &l, std::vector<Need> &out) {
     const uint64_t cache = slots * kvh * cap * hd * T;
     const uint64_t chunks = attn_chunks((uint32_t)cap);
     const uint64_t table = cap * (hd / 2) * F;
+    auto some = [](const char *name, uint64_t bytes) { return Need{name, std::max<uint64_t>(bytes, 16), bytes == 0}; };
     switch (l.kernel) {
         case TG_KERNEL_RMSNORM:
             out = {{"x", rows * H * F}, {"gain", H * F}, {"out", rows * H * F}};
@@ -180,6 +183,27 @@ static int needs(const Launch &l, std::vector<Need> &out) {
             out = {{"h", rows * 2 * cap * p.k * 2}, {"W", (uint64_t)p.feat * p.k * 2}, {"bias", (uint64_t)p.feat * 2},
                    {"sampling", rows * 2 * F}, {"x", rows * p.feat * p.frames * F}};
             break;
+        // A paged batch; arrays that may be empty are bound as any 16 bytes.
+        case TG_KERNEL_PAGE_PLAN:
+            out = {{"held", (uint64_t)p.seqs * 4}, {"fresh", (uint64_t)p.seqs * 4}, some("free", (uint64_t)p.n * 4),
+                   {"table", (uint64_t)p.seqs * p.stride * 4}, {"at", 2 * rows * 4}, {"place", rows * 4},
+                   {"starts", ((uint64_t)p.seqs + 1) * 4}, {"next", (uint64_t)p.seqs * 4}, {"counts", 16}};
+            break;
+        case TG_KERNEL_ROPE_PAGES:
+            out = {{"at", 2 * rows * 4}, {"place", rows * 4}, {"c", rows * width * (p.flags & 2 ? T : F)},
+                   some("cos", (uint64_t)p.n * (p.k / 2) * F), some("sin", (uint64_t)p.n * (p.k / 2) * F),
+                   {"q", rows * attn * T}, {"k_pages", cache}, {"v_pages", cache}};
+            break;
+        case TG_KERNEL_ATTENTION_PAGES:
+            out = {{"q", rows * attn * T}, {"k_pages", cache}, {"v_pages", cache}, {"at", 2 * rows * 4},
+                   {"table", (uint64_t)p.seqs * p.stride * 4}, some("shared", (p.first + cap - 1) / cap * 4),
+                   {"work", attention_pages_work(p)}, {"out", rows * attn * T}};
+            break;
+        case TG_KERNEL_LOGITS_PICK:
+            out = {{"logits", rows * p.stride * T}, some("seen", (uint64_t)p.k * 4), {"spans", rows * 24},
+                   {"penalties", rows * 12}, some("bias_ids", (uint64_t)p.k1 * 4), some("bias", (uint64_t)p.k1 * 4),
+                   some("masks", (uint64_t)p.m * ((p.n + 31ull) / 32) * 4), {"out", rows * p.stride * T}, {"pick", rows * 4}};
+            break;
         default:
             return fail(TG_EINVAL, "no kernel %u", l.kernel);
     }
@@ -192,7 +216,7 @@ static const char *kernel_name(uint32_t k) {
         "gemv_gate_up", "stream_read", "norm_rows", "add_norm_rows", "rope_rows", "attention_rows",
         "silu_mul_rows", "gemm", "(unused)", "gemm_silu", "attention_rows_tc", "gemm_qkv_rope", "gemv_linear",
         "local_norm", "local_partial", "local_gate_up", "local_attention", "local_add_norm", "local_rows",
-        "local_embed", "cfm_noise", "dit_euler"};
+        "local_embed", "cfm_noise", "dit_euler", "page_plan", "rope_pages", "attention_pages", "logits_pick"};
     return k < TG_KERNEL_COUNT ? names[k] : "?";
 }
 
@@ -242,12 +266,81 @@ static int check_local_shape(const Launch &l) {
     return TG_OK;
 }
 
+// A paged batch's shape rules.
+static bool is_paged(uint32_t k) { return k >= TG_KERNEL_PAGE_PLAN && k <= TG_KERNEL_LOGITS_PICK; }
+
+static int check_paged_shape(const Launch &l) {
+    const tg_params &p = l.p;
+    const char *name = kernel_name(l.kernel);
+    if (p.rows == 0) return fail(TG_ESHAPE, "%s: 0 rows", name);
+    if (l.kernel == TG_KERNEL_LOGITS_PICK) {
+        if (p.n == 0 || p.n > 0x7fffffffu || p.stride < p.n || p.rows > 65535)
+            return fail(TG_ESHAPE, "logits_pick: %u tokens in rows of %u, %u rows (1 to 2^31 - 1 tokens, at most 65535 rows)",
+                        p.n, p.stride, p.rows);
+        return TG_OK;
+    }
+    if (p.capacity == 0 || p.capacity % PAGE_STEP || p.slots == 0 || (uint64_t)p.capacity * p.slots >= TG_SPARE)
+        return fail(TG_ESHAPE, "%s: %u pages of %u positions (a multiple of %u, fewer than 2^32 - 1 positions in all)", name,
+                    p.slots, p.capacity, PAGE_STEP);
+    if (l.kernel == TG_KERNEL_PAGE_PLAN) {
+        if (p.seqs == 0 || p.seqs > PLAN_MAX_SEQS || p.stride == 0 || p.rows > 0x7fffffffu)
+            return fail(TG_ESHAPE, "page_plan: %u requests (1 to %u), tables of %u pages, %u rows", p.seqs, PLAN_MAX_SEQS,
+                        p.stride, p.rows);
+        return TG_OK;
+    }
+    if (p.kv_heads == 0 || p.heads == 0 || p.heads % p.kv_heads || p.heads / p.kv_heads > MAX_GROUP ||
+        (p.head_dim != 64 && p.head_dim != 128) || p.heads > 1024)
+        return fail(TG_ESHAPE, "%s: %u heads over %u of %u (at most %u to a KV head, 64 or 128 wide)", name, p.heads,
+                    p.kv_heads, p.head_dim, MAX_GROUP);
+    if (l.kernel == TG_KERNEL_ROPE_PAGES) {
+        if (p.flags > 3 || (p.rope ? (p.k == 0 || p.k % 2 || p.k > p.head_dim || p.n == 0) : p.k != 0) || p.rows > 0x7fffffffu)
+            return fail(TG_ESHAPE, "rope_pages: %u of %u dimensions rotated (even; 0 without rope), %u positions, flags %u", p.k,
+                        p.head_dim, p.n, p.flags);
+        return TG_OK;
+    }
+    if (p.seqs == 0 || p.stride == 0 || p.rows > 65535 || (uint64_t)p.first + (uint64_t)p.stride * p.capacity >= TG_SPARE)
+        return fail(TG_ESHAPE, "attention_pages: %u rows (at most 65535) of %u requests, %u shared positions, tables of %u pages",
+                    p.rows, p.seqs, p.first, p.stride);
+    return TG_OK;
+}
+
+// The bindings a paged kernel writes, as bits.
+static uint32_t paged_outputs(uint32_t k) {
+    switch (k) {
+        case TG_KERNEL_PAGE_PLAN: return 0x1f8;        // table, at, place, starts, next, counts
+        case TG_KERNEL_ROPE_PAGES: return 0xe0;        // q, k, v
+        case TG_KERNEL_ATTENTION_PAGES: return 0xc0;   // work, out
+        case TG_KERNEL_LOGITS_PICK: return 0x180;      // out, pick
+        default: return 0;
+    }
+}
+
+// An output that overlaps another binding is refused: the kernels' blocks read and write in no order.
+// logits_pick's out may be exactly its logits (a value is read and written by one thread).
+static int check_paged_overlap(const Launch &l, const std::vector<Need> &need) {
+    const uint32_t outs = paged_outputs(l.kernel);
+    for (size_t i = 0; i < need.size(); i++) {
+        if (!(outs >> i & 1)) continue;
+        const char *a = static_cast<const char *>(l.ptr[i]);
+        for (size_t j = 0; j < need.size(); j++) {
+            if (j == i || need[j].empty || (l.kernel == TG_KERNEL_LOGITS_PICK && i == 7 && j == 0 && l.ptr[i] == l.ptr[j])) continue;
+            const char *b = static_cast<const char *>(l.ptr[j]);
+            if (a < b + need[j].bytes && b < a + need[i].bytes)
+                return fail(TG_EINVAL, "%s: binding %zu (%s) overlaps binding %zu (%s)", kernel_name(l.kernel), i,
+                            need[i].name, j, need[j].name);
+        }
+    }
+    return TG_OK;
+}
+
 // Shapes the kernels cannot cover exactly are refused (decode.rs:468-491, prefill.rs:233-262).
 static int check_shape(const Launch &l) {
     const tg_params &p = l.p;
     if (is_local(l.kernel)) return check_local_shape(l);
+    if (l.kernel == TG_KERNEL_PAGE_PLAN) return check_paged_shape(l);
     if (p.dtype != TG_F32 && p.dtype != TG_BF16) return fail(TG_ESHAPE, "dtype %u", p.dtype);
     const uint32_t vec = p.dtype == TG_BF16 ? 256 : 128;  // a warp's 16-byte step over K
+    if (is_paged(l.kernel)) return check_paged_shape(l);
     auto heads_ok = [&] {
         return p.kv_heads > 0 && p.heads % p.kv_heads == 0 && p.heads / p.kv_heads <= MAX_GROUP &&
                (p.head_dim == 64 || p.head_dim == 128) && p.capacity > 0 && p.capacity % CAPACITY_STEP == 0;
@@ -370,7 +463,7 @@ int check_launch(const Launch &l0) {
                         kernel_name(l.kernel), i, need[i].name, (unsigned long long)l.bytes[i],
                         (unsigned long long)need[i].bytes);
     }
-    return TG_OK;
+    return is_paged(l.kernel) ? check_paged_overlap(l, need) : TG_OK;
 }
 
 int enqueue_launch(const Launch &l, uint32_t *err, cudaStream_t s, int sm_count) {
@@ -424,6 +517,10 @@ int enqueue_launch(const Launch &l, uint32_t *err, cudaStream_t s, int sm_count)
         case TG_KERNEL_LOCAL_EMBED: e = launch_local_embed(p, F(0), b[1], b[2], b[3], b[4], s); break;
         case TG_KERNEL_CFM_NOISE: e = launch_cfm_noise(p, F(0), F(1), F(2), s); break;
         case TG_KERNEL_DIT_EULER: e = launch_dit_euler(p, b[0], b[1], b[2], F(3), F(4), s); break;
+        case TG_KERNEL_PAGE_PLAN: e = launch_page_plan(p, U(0), U(1), U(2), U(3), U(4), U(5), U(6), U(7), U(8), err, s); break;
+        case TG_KERNEL_ROPE_PAGES: e = launch_rope_pages(p, U(0), U(1), b[2], F(3), F(4), b[5], b[6], b[7], err, s); break;
+        case TG_KERNEL_ATTENTION_PAGES: e = launch_attention_pages(p, b[0], b[1], b[2], U(3), U(4), U(5), b[6], b[7], err, s); break;
+        case TG_KERNEL_LOGITS_PICK: e = launch_logits_pick(p, b[0], U(1), U(2), F(3), U(4), F(5), U(6), b[7], U(8), err, s); break;
         default: return fail(TG_EINVAL, "no kernel %u", l.kernel);
     }
     if (e != cudaSuccess)
@@ -641,8 +738,30 @@ extern "C" int tg_mem_alloc(tg_ctx *ctx, uint64_t bytes, tg_residence residence,
     return TG_OK;
 }
 
+extern "C" int tg_mem_wrap(tg_ctx *ctx, void *ptr, uint64_t bytes, tg_mem **out) {
+    if (!ctx || !ptr || !out) return fail(TG_EINVAL, "tg_mem_wrap: null argument");
+    *out = nullptr;
+    if (bytes == 0) return fail(TG_EINVAL, "tg_mem_wrap: 0 bytes");
+    cudaPointerAttributes a;
+    TG_CUDA(cudaPointerGetAttributes(&a, ptr));
+    if (a.type != cudaMemoryTypeDevice || a.device != ctx->device)
+        return fail(TG_EINVAL, "tg_mem_wrap: not memory of device %d", ctx->device);
+    tg_mem *m = new (std::nothrow) tg_mem();
+    if (!m) return TG_ENOMEM;
+    m->ctx = ctx;
+    m->ptr = ptr;
+    m->bytes = bytes;
+    m->owned = false;
+    *out = m;
+    return TG_OK;
+}
+
 extern "C" int tg_mem_free(tg_mem *m) {
     if (!m) return TG_OK;
+    if (!m->owned) {
+        delete m;
+        return TG_OK;
+    }
     cudaSetDevice(m->ctx->device);
     if (m->residence == TG_RES_DEVICE)
         cudaFree(m->ptr);
@@ -724,6 +843,7 @@ extern "C" int tg_copy_regions(tg_ctx *ctx, tg_mem *src, tg_mem *dst, const tg_r
 static int resolve(const tg_dispatch &d, Launch &l) {
     if (!d.params) return fail(TG_EINVAL, "dispatch of kernel %u without params", d.kernel);
     if (d.n_bindings && !d.bindings) return fail(TG_EINVAL, "dispatch of kernel %u: null bindings", d.kernel);
+    if (d.n_bindings > 64) return fail(TG_EINVAL, "dispatch of kernel %u: %u bindings", d.kernel, d.n_bindings);
     l.kernel = d.kernel;
     l.p = *d.params;
     l.label = d.label ? d.label : "";
@@ -770,6 +890,57 @@ extern "C" int tg_dispatch_once(tg_ctx *ctx, const tg_dispatch *d, double *ns) {
     cudaEventDestroy(e0);
     cudaEventDestroy(e1);
     return st;
+}
+
+namespace {
+// The calling thread's current device, put back at the end of a call that changes it.
+struct DeviceGuard {
+    int before = -1;
+    explicit DeviceGuard(int device) {
+        int now = -1;
+        if (cudaGetDevice(&now) == cudaSuccess && now != device && cudaSetDevice(device) == cudaSuccess) before = now;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+}  // namespace
+
+extern "C" int tg_dispatch_enqueue(tg_ctx *ctx, const tg_dispatch *d, void *stream) try {
+    if (!ctx || !d) return fail(TG_EINVAL, "tg_dispatch_enqueue: null argument");
+    Launch l;
+    int st = resolve(*d, l);
+    if (!st) st = check_launch(l);
+    if (st) return st;
+    for (uint32_t i = 0; i < d->n_bindings; i++)
+        if (d->bindings[i].mem->ctx->device != ctx->device)
+            return fail(TG_EINVAL, "tg_dispatch_enqueue: binding %u is on device %d, the context on %d", i,
+                        d->bindings[i].mem->ctx->device, ctx->device);
+    // A stream of another device than the current one refuses the launch itself (cudaStreamGetDevice
+    // would say so first, but not while the stream is being captured).
+    const DeviceGuard guard(ctx->device);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return enqueue_launch(l, ctx->err_dev, s, ctx->sm_count);
+} catch (const std::bad_alloc &) {
+    return TG_ENOMEM;  // host memory for the dispatch's bindings; no message, which would need some too
+}
+
+extern "C" int tg_dispatch_needs(uint32_t kernel, const tg_params *p, uint64_t *bytes, size_t n, size_t *count) try {
+    if (!p || !count || (n && !bytes)) return fail(TG_EINVAL, "tg_dispatch_needs: null argument");
+    *count = 0;
+    if (kernel >= TG_KERNEL_COUNT) return fail(TG_EINVAL, "no kernel %u", kernel);
+    Launch l;
+    l.kernel = kernel;
+    l.p = *p;
+    std::vector<Need> need;
+    int st = check_shape(l);
+    if (!st) st = needs(l, need);
+    if (st) return st;
+    for (size_t i = 0; i < need.size() && i < n; i++) bytes[i] = need[i].bytes;
+    *count = need.size();
+    return TG_OK;
+} catch (const std::bad_alloc &) {
+    return TG_ENOMEM;
 }
 
 extern "C" int tg_program_create(tg_ctx *ctx, const tg_dispatch *ds, size_t n, int timed, tg_program **out) {

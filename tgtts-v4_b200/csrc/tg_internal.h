@@ -31,6 +31,7 @@ struct tg_mem {
     void *host = nullptr; // pinned host address for UPLOAD / READBACK
     uint64_t bytes = 0;
     tg_residence residence = TG_RES_DEVICE;
+    bool owned = true;  // false: tg_mem_wrap's, the memory is the caller's
 };
 
 namespace tg {
@@ -232,6 +233,23 @@ cudaError_t launch_gemm_qkv_rope(const tg_params &p, const void *a, const void *
 // out[m][n / 2] = SiLU(gate) up of C = A B^T, B's rows in gate_up_row's order (bf16, n % 256 == 0).
 cudaError_t launch_gemm_silu(const tg_params &p, const void *a, const void *b, void *out, uint32_t *err,
                              cudaStream_t s);
+
+// A paged, prefix-sharing batch (kernels_paged.cu, attention_pages.cu).
+constexpr uint32_t PAGE_STEP = 16;           // a page's positions are a multiple of this
+constexpr uint32_t PLAN_MAX_SEQS = 16384;    // page_plan's requests: its two sums of each in shared memory
+cudaError_t launch_page_plan(const tg_params &p, const uint32_t *held, const uint32_t *fresh, const uint32_t *free,
+                             uint32_t *table, uint32_t *at, uint32_t *place, uint32_t *starts, uint32_t *next,
+                             uint32_t *counts, uint32_t *err, cudaStream_t s);
+cudaError_t launch_rope_pages(const tg_params &p, const uint32_t *at, const uint32_t *place, const void *c,
+                              const float *cosv, const float *sinv, void *q, void *k, void *v, uint32_t *err,
+                              cudaStream_t s);
+cudaError_t launch_attention_pages(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at,
+                                   const uint32_t *table, const uint32_t *shared, void *work, void *out, uint32_t *err,
+                                   cudaStream_t s);
+uint64_t attention_pages_work(const tg_params &p);
+cudaError_t launch_logits_pick(const tg_params &p, const void *logits, const uint32_t *seen, const uint32_t *spans,
+                               const float *penalties, const uint32_t *bias_ids, const float *bias,
+                               const uint32_t *masks, void *out, uint32_t *pick, uint32_t *err, cudaStream_t s);
 
 // The local stacks (local.cu): f16 kernels over m tokens in sequences of p.capacity.
 bool local_proj_supported(int M, int N, int K, int parts);
