@@ -31,7 +31,8 @@ __host__ __device__ inline uint64_t all_pieces(const tg_params &p) {
     return shared_pieces(p.first) + ((uint64_t)p.stride * p.capacity + own_piece(p.head_dim) - 1) / own_piece(p.head_dim);
 }
 
-// The partials in the work buffer: o f32 [rows][heads][pieces][hd], then m, l f32 [rows][heads][pieces][2].
+// The partials in the work buffer, from its first 256-byte boundary: o f32 [rows][heads][pieces][hd], then
+// m, l f32 [rows][heads][pieces][2].
 struct Partials {
     float *o, *ml;
 };
@@ -376,6 +377,13 @@ TG_DEVICE uint64_t mn_desc(uint32_t addr, uint32_t chunk) {
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
+// 32 aligned bytes in one store: a whole sector.
+TG_DEVICE void store8(float *dst, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 template <int HD>
 __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
     prefix_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -443,28 +451,35 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
                     tma_load_3d(base + C::Q + h * C::TILE + c * C::HALF, &qmap, c * 64, kv * group, (tile0 + h) * tile_rows, B(bq));
         }
         // A lane to a copy: one half of the dimensions, one box of positions. Keys run a tile ahead of
-        // values, as their stages come free earlier.
+        // values, as their stages come free earlier, and the pages' numbers a tile ahead of the keys.
         const int boxes = 128 / (int)box, seg = lane % boxes, half = lane / boxes;
-        auto load = [&](int j, uint32_t dst, const CUtensorMap *map, uint64_t *full, uint64_t *empty) {
-            const int b = j % C::STAGES, live = min(128, (int)keys - j * 128), segs = (live + (int)box - 1) / (int)box;
-            const uint32_t pos = begin + j * 128 + seg * box;
-            const bool mine = half < C::HALVES && seg < segs;
-            uint32_t id = mine ? __ldg(shared + pos / p.capacity) : 0u;
+        auto page_of = [&](int j) {
+            const uint32_t in = j * 128 + seg * box;
+            uint32_t id = in < keys ? __ldg(shared + (begin + in) / p.capacity) : 0u;
             if (id >= p.slots) {
                 atomicExch(err, ERR_BAD_INDEX);
                 id = 0;
             }
+            return id;
+        };
+        auto load = [&](int j, uint32_t id, uint32_t dst, const CUtensorMap *map, uint64_t *full, uint64_t *empty) {
+            const int b = j % C::STAGES, live = min(128, (int)keys - j * 128), segs = (live + (int)box - 1) / (int)box;
+            const uint32_t pos = begin + j * 128 + seg * box;
             mbar_wait(B(empty[b]), ((j / C::STAGES) & 1) ^ 1, err, &gave_up);
             if (lane == 0) mbar_arrive_expect_tx(B(full[b]), C::HALVES * segs * box * 128);
             __syncwarp();
-            if (mine)
+            if (half < C::HALVES && seg < segs)
                 tma_load_3d(base + dst + b * C::TILE + half * C::HALF + seg * box * 128, map, half * 64, (int)(pos % p.capacity),
                             (int)(id * kvh + kv), B(full[b]));
         };
-        load(0, C::K, &kmap, bk_full, bk_empty);
+        uint32_t id = page_of(0), id1 = page_of(1);
+        load(0, id, C::K, &kmap, bk_full, bk_empty);
         for (int j = 0; j < n; j++) {
-            if (j + 1 < n) load(j + 1, C::K, &kmap, bk_full, bk_empty);
-            load(j, C::V, &vmap, bv_full, bv_empty);
+            const uint32_t id2 = page_of(j + 2);
+            if (j + 1 < n) load(j + 1, id1, C::K, &kmap, bk_full, bk_empty);
+            load(j, id, C::V, &vmap, bv_full, bv_empty);
+            id = id1;
+            id1 = id2;
         }
         // Every copy has landed before the block can end.
         for (int j = n > C::STAGES ? n - C::STAGES : 0; j < n; j++) {
@@ -552,7 +567,7 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
 #pragma unroll
                 for (int e = 0; e < 4; e++) sum4[e] = make_float2(0.0f, 0.0f);
                 float mxs[2] = {-INFINITY, -INFINITY};
-                const float nm = mref != -INFINITY ? -mref : -INFINITY;  // no reference yet: P comes out 0
+                const float nm = mref != -INFINITY ? -mref : -INFINITY;  // every score -inf: P comes out 0
                 const float2 scale22 = make_float2(scale2, scale2), neg_m = make_float2(nm, nm);
 #pragma unroll
                 for (int c2 = 0; c2 < 2; c2++) {
@@ -588,26 +603,42 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
                 return ((sum4[0].x + sum4[0].y) + (sum4[1].x + sum4[1].y)) +
                        ((sum4[2].x + sum4[2].y) + (sum4[3].x + sum4[3].y));
             };
+            if (j == 0) {  // no reference yet: the tile's maximum first
+                float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c4 = 0; c4 < 2; c4++) {
+                    uint32_t r[4][16];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) tmem_ld16_nowait(lanes + C::s_col(h, 0) + (uint32_t)(c4 * 64 + c * 16), r[c]);
+                    tmem_wait_ld();
+                    const int in = min(live - c4 * 64, 64);
+#pragma unroll
+                    for (int c = 0; c < 64; c += 2)
+                        mxs[(c / 2) % 4] = max3(mxs[(c / 2) % 4], c < in ? __uint_as_float(r[c / 16][c % 16]) : -INFINITY,
+                                                c + 1 < in ? __uint_as_float(r[c / 16][c % 16 + 1]) : -INFINITY);
+                }
+                mref = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * scale2;
+            }
             float a = 1.0f, mx;
             float sum = p_pass(mx, true);
             const float m_tile = mx * scale2;
-            const bool move = m_tile != -INFINITY && (mref == -INFINITY || m_tile > mref + MOVE_PAST);
+            const bool move = m_tile > mref + MOVE_PAST;
             if (__any_sync(0xffffffffu, move)) {
+                // A query of the warp moves: O (with PV_{j-1} in it) rescaled, a query that keeps its
+                // reference times 1, then the warp's P_j again from S_j, still in TMEM.
                 a = move && mref != -INFINITY ? hw_exp2(mref - m_tile) : 1.0f;
                 if (move) mref = m_tile;
                 tmem_wait_st();
-                if (__any_sync(0xffffffffu, a != 1.0f)) {
 #pragma unroll
-                    for (int c = 0; c < HD / 16; c++) {
-                        uint32_t o[16];
-                        tmem_ld16_nowait(lanes + C::o_col(h) + c * 16, o);
-                        tmem_wait_ld();
+                for (int c = 0; c < HD / 16; c++) {
+                    uint32_t o[16];
+                    tmem_ld16_nowait(lanes + C::o_col(h) + c * 16, o);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-                        tmem_st16(lanes + C::o_col(h) + c * 16, o);
-                    }
-                    tmem_wait_st();
+                    for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+                    tmem_st16(lanes + C::o_col(h) + c * 16, o);
                 }
+                tmem_wait_st();
                 sum = p_pass(mx, false);
             }
             tmem_wait_st();
@@ -626,10 +657,10 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
             uint32_t o[16];
             tmem_ld16_nowait(lanes + C::o_col(h) + c * 16, o);
             tmem_wait_ld();
-            if (real)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    *reinterpret_cast<uint4 *>(out.o + to * HD + c * 16 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            if (real) {
+                store8(out.o + to * HD + c * 16, o);
+                store8(out.o + to * HD + c * 16 + 8, o + 8);
+            }
         }
         if (real) *reinterpret_cast<float2 *>(out.ml + to * 2) = make_float2(mref, l);
     }
@@ -640,36 +671,55 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
 }
 
 // Joins a row's partials, a warp to a head, in piece order. References are in base 2 for bf16, natural for f32.
+// A lane takes four dimensions of every LANES-th piece, so that a warp has several pieces' loads in flight; the
+// lanes' sums are added by a butterfly.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128)
     join_kernel(tg_params p, const uint32_t *__restrict__ at, Partials in, uint32_t np, uint32_t pieces, T *__restrict__ out) {
-    constexpr int D = HD / 32;
+    constexpr int LANES = 32 / (HD / 4);  // pieces at once
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, d = 4 * (lane % (HD / 4)), of = lane / (HD / 4);
     const uint64_t item = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (item >= (uint64_t)p.rows * p.heads) return;
-    const int row = (int)(item / p.heads);
     uint32_t length, seq;
-    if (!paged_row(p, at, row, length, seq, nullptr)) return;
+    if (!paged_row(p, at, (int)(item / p.heads), length, seq, nullptr)) return;
     const uint32_t n = np + (length + own_piece(HD) - 1) / own_piece(HD);
     const float2 *ml = reinterpret_cast<const float2 *>(in.ml) + item * pieces;
-    const float *o = in.o + item * pieces * HD + lane * D;
-    float m = -INFINITY;
-    for (uint32_t i = lane; i < n; i += 32) m = fmaxf(m, ml[i].x);
-    m = warp_max(m);
-    float l = 0.0f, acc[D];
-#pragma unroll
-    for (int d = 0; d < D; d++) acc[d] = 0.0f;
-    for (uint32_t i = 0; i < n; i++) {
-        const float2 part = ml[i];
-        const float e = part.x == -INFINITY ? 0.0f : sizeof(T) == 2 ? exp2f(part.x - m) : expf(part.x - m);
-        l = __fmaf_rn(part.y, e, l);
-#pragma unroll
-        for (int d = 0; d < D; d++) acc[d] = __fmaf_rn(o[(size_t)i * HD + d], e, acc[d]);
+    const float *o = in.o + item * pieces * HD + d;
+    float m = -INFINITY, l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto power = [](float x) { return sizeof(T) == 2 ? exp2f(x) : expf(x); };
+    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+        // 32 pieces at once: a lane holds one's reference and sum.
+        const float2 part = i0 + lane < n ? ml[i0 + lane] : make_float2(-INFINITY, 0.0f);
+        const float next = fmaxf(m, warp_max(part.x)), keep = m == -INFINITY ? 0.0f : power(m - next);
+        const float e = part.x == -INFINITY ? 0.0f : power(part.x - next);
+        m = next;
+        l = __fmaf_rn(l, keep, warp_sum(part.y * e));
+        acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+        const uint32_t count = min(n - i0, 32u);
+#pragma unroll 4
+        for (uint32_t i = 0; i < count; i += LANES) {
+            const float w = __shfl_sync(0xffffffffu, e, (i + of) & 31);
+            if (i + of >= count) continue;
+            const float4 x = *reinterpret_cast<const float4 *>(o + (size_t)(i0 + i + of) * HD);
+            acc = make_float4(__fmaf_rn(x.x, w, acc.x), __fmaf_rn(x.y, w, acc.y), __fmaf_rn(x.z, w, acc.z), __fmaf_rn(x.w, w, acc.w));
+        }
     }
-#pragma unroll
-    for (int d = 0; d < D; d++) out[item * HD + lane * D + d] = from_f32<T>(__fdiv_rn(acc[d], l));
+    if (LANES > 1) {
+        acc.x += __shfl_xor_sync(0xffffffffu, acc.x, 16);
+        acc.y += __shfl_xor_sync(0xffffffffu, acc.y, 16);
+        acc.z += __shfl_xor_sync(0xffffffffu, acc.z, 16);
+        acc.w += __shfl_xor_sync(0xffffffffu, acc.w, 16);
+    }
+    if (of) return;
+    T *dst = out + item * HD + d;
+    const float4 r = make_float4(__fdiv_rn(acc.x, l), __fdiv_rn(acc.y, l), __fdiv_rn(acc.z, l), __fdiv_rn(acc.w, l));
+    if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(fa::pack_bf16(r.x, r.y), fa::pack_bf16(r.z, r.w));
+    else
+        *reinterpret_cast<float4 *>(dst) = r;
 }
 
 // A 3-D map over bf16 [outer][rows][hd]: boxes of 64 dimensions x `box_rows` x `box_outer` in the 128-byte
@@ -689,7 +739,8 @@ cudaError_t attend(const tg_params &p, const void *q, const void *k, const void 
                    const uint32_t *shared, void *work, void *out, uint32_t *err, cudaStream_t s) {
     const uint64_t pieces = all_pieces(p), items = (uint64_t)p.rows * p.heads;
     if (pieces > 0x7fffffffu || p.kv_heads > 65535) return cudaErrorNotSupported;
-    Partials part{static_cast<float *>(work), static_cast<float *>(work) + items * pieces * HD};
+    float *o = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(work) + 255) & ~uintptr_t(255));
+    Partials part{o, o + items * pieces * HD};
     const uint32_t np = shared_pieces(p.first);
     cudaError_t e = cudaSuccess;
     if constexpr (sizeof(T) == 2) {
@@ -725,7 +776,7 @@ cudaError_t attend(const tg_params &p, const void *q, const void *k, const void 
 
 uint64_t attention_pages_work(const tg_params &p) {
     if (p.head_dim == 0 || p.head_dim > 16384) return 0;
-    return (uint64_t)p.rows * p.heads * all_pieces(p) * (p.head_dim + 2) * sizeof(float);
+    return (uint64_t)p.rows * p.heads * all_pieces(p) * (p.head_dim + 2) * sizeof(float) + 256;
 }
 
 cudaError_t launch_attention_pages(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at,

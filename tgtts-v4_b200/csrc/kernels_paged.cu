@@ -4,6 +4,8 @@
 // bound by memory or by their launch: one launch each, every input read once from HBM.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "tg_common.cuh"
 #include "tg_internal.h"
 
@@ -160,22 +162,29 @@ TG_DEVICE void turn(float &a, float &b, float co, float si) {
     a = na;
 }
 
+// Division by a number the host knows: n / d = (mulhi(n, mul) + n) >> shift for every 32-bit n
+// (Granlund and Montgomery, "Division by invariant integers using multiplication").
+struct Divisor {
+    uint32_t d, mul, shift;
+    explicit Divisor(uint32_t by) : d(by), shift(0) {
+        while ((1ull << shift) < by) shift++;
+        mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
+    }
+    TG_DEVICE uint32_t div(uint32_t n) const { return (uint32_t)(((uint64_t)__umulhi(n, mul) + n) >> shift); }
+};
+
 // Where a row's head is stored: null when the row does not write it.
 template <typename T>
-TG_DEVICE T *rope_out(const tg_params &p, int row, int head, uint32_t to, T *q, T *k, T *v) {
-    if (head < (int)p.heads) return q + ((size_t)row * p.heads + head) * p.head_dim;
+TG_DEVICE T *rope_out(const tg_params &p, const Divisor &page, uint32_t row, uint32_t head, uint32_t to, T *q, T *k, T *v) {
+    if (head < p.heads) return q + ((size_t)row * p.heads + head) * p.head_dim;
     if (to == SPARE) return nullptr;
-    const int h = head - (int)p.heads;
-    T *cache = h < (int)p.kv_heads ? k : v;
-    const uint32_t page = to / p.capacity, off = to % p.capacity;
-    return cache + (((size_t)page * p.kv_heads + h % (int)p.kv_heads) * p.capacity + off) * p.head_dim;
+    const bool value = head >= p.heads + p.kv_heads;
+    const uint32_t id = page.div(to), off = to - id * p.capacity, h = head - p.heads - (value ? p.kv_heads : 0);
+    return (value ? v : k) + (((size_t)id * p.kv_heads + h) * p.capacity + off) * p.head_dim;
 }
 
-// A row's position and place; false when it writes nothing.
-TG_DEVICE bool rope_row(const tg_params &p, const uint32_t *at, const uint32_t *place, int row, uint32_t &pos,
-                        uint32_t &to, uint32_t *err) {
-    pos = at[row];
-    to = place[row];
+// False for a row that writes nothing.
+TG_DEVICE bool rope_row(const tg_params &p, uint32_t pos, uint32_t to, uint32_t *err) {
     if (pos == SPARE) return false;
     if ((p.rope && pos >= p.n) || (to != SPARE && to >= p.slots * p.capacity)) {
         atomicExch(err, ERR_BAD_INDEX);
@@ -184,79 +193,114 @@ TG_DEVICE bool rope_row(const tg_params &p, const uint32_t *at, const uint32_t *
     return true;
 }
 
-// Eight dimensions of a head to a thread, for a rotated part that is a multiple of 8: rotated ones as
-// four pairs (in the half layout two runs of four, each a warp's whole sectors).
+// For a rotated part that is a multiple of 8: eight dimensions of two heads of a row to a thread (heads h
+// and h + half the heads, which turn by the same angles), rotated ones as four pairs (in the half layout
+// two runs of four, each a warp's whole sectors). All of a thread's loads of c leave before the first is
+// used, and before it knows whether its row is spare. A block takes ROPE_ROWS x the row's threads.
+constexpr int ROPE_THREADS = 256;
+
 template <typename T, typename C, bool INTER>
-__global__ void __launch_bounds__(256)
-    rope_pages_kernel(tg_params p, const uint32_t *__restrict__ at, const uint32_t *__restrict__ place,
-                      const C *__restrict__ c, const float *__restrict__ cosv, const float *__restrict__ sinv,
-                      T *__restrict__ q, T *__restrict__ k, T *__restrict__ v, uint32_t *err) {
+__global__ void __launch_bounds__(ROPE_THREADS)
+    rope_pages_kernel(tg_params p, Divisor page, Divisor row_units, uint32_t block_rows, const uint32_t *__restrict__ at,
+                      const uint32_t *__restrict__ place, const C *__restrict__ c, const float *__restrict__ cosv,
+                      const float *__restrict__ sinv, T *__restrict__ q, T *__restrict__ k, T *__restrict__ v, uint32_t *err) {
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t units = p.head_dim / 8, heads = p.heads + 2 * p.kv_heads, row_units = units * heads;
-    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (uint64_t)p.rows * row_units) return;
-    const uint32_t row = (uint32_t)(i / row_units), in_row = (uint32_t)(i % row_units), head = in_row / units, u = in_row % units;
-    uint32_t pos, to;
-    if (!rope_row(p, at, place, row, pos, to, err)) return;
-    T *o = rope_out(p, row, head, to, q, k, v);
-    if (!o) return;
-    const C *x = c + ((size_t)row * heads + head) * p.head_dim;
-    const bool turned = p.rope && head < p.heads + p.kv_heads && u < p.k / 8;
-    const uint32_t d0 = (turned && !INTER) ? 4 * u : 8 * u, d1 = (turned && !INTER) ? p.k / 2 + 4 * u : 8 * u + 4;
-    float4 a = load4(x + d0), b = load4(x + d1);
-    if (turned) {
-        const float4 co = __ldg(reinterpret_cast<const float4 *>(cosv + (size_t)pos * (p.k / 2)) + u);
-        const float4 si = __ldg(reinterpret_cast<const float4 *>(sinv + (size_t)pos * (p.k / 2)) + u);
-        if (INTER) {
-            turn(a.x, a.y, co.x, si.x);
-            turn(a.z, a.w, co.y, si.y);
-            turn(b.x, b.y, co.z, si.z);
-            turn(b.z, b.w, co.w, si.w);
-        } else {
-            turn(a.x, b.x, co.x, si.x);
-            turn(a.y, b.y, co.y, si.y);
-            turn(a.z, b.z, co.z, si.z);
-            turn(a.w, b.w, co.w, si.w);
+    const uint32_t units = p.head_dim / 8, heads = p.heads + 2 * p.kv_heads, apart = (heads + 1) / 2;
+    const uint32_t row0 = blockIdx.x * block_rows, here = min(block_rows, p.rows - row0) * row_units.d;
+    for (uint32_t i = threadIdx.x; i < here; i += ROPE_THREADS) {
+        const uint32_t in_block = row_units.div(i), row = row0 + in_block, in_row = i - in_block * row_units.d;
+        const uint32_t u = in_row % units, head0 = in_row / units, head1 = head0 + apart;  // units: 8 or 16
+        const uint32_t pos = at[row], to = place[row];
+        const bool rotated = p.rope && u < p.k / 8;
+        float4 a[2], b[2];
+        uint32_t d0[2], d1[2];
+        bool turned[2];
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            const uint32_t head = n ? head1 : head0;
+            turned[n] = rotated && head < p.heads + p.kv_heads;
+            d0[n] = (turned[n] && !INTER) ? 4 * u : 8 * u;
+            d1[n] = (turned[n] && !INTER) ? p.k / 2 + 4 * u : 8 * u + 4;
+            if (head >= heads) continue;
+            const C *x = c + ((size_t)row * heads + head) * p.head_dim;
+            a[n] = load4(x + d0[n]);
+            b[n] = load4(x + d1[n]);
+        }
+        if (!rope_row(p, pos, to, err)) continue;
+        float4 co, si;
+        if (turned[0] || turned[1]) {
+            co = __ldg(reinterpret_cast<const float4 *>(cosv + (size_t)pos * (p.k / 2)) + u);
+            si = __ldg(reinterpret_cast<const float4 *>(sinv + (size_t)pos * (p.k / 2)) + u);
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            const uint32_t head = n ? head1 : head0;
+            if (head >= heads) continue;
+            T *o = rope_out(p, page, row, head, to, q, k, v);
+            if (!o) continue;
+            if (turned[n]) {
+                if (INTER) {
+                    turn(a[n].x, a[n].y, co.x, si.x);
+                    turn(a[n].z, a[n].w, co.y, si.y);
+                    turn(b[n].x, b[n].y, co.z, si.z);
+                    turn(b[n].z, b[n].w, co.w, si.w);
+                } else {
+                    turn(a[n].x, b[n].x, co.x, si.x);
+                    turn(a[n].y, b[n].y, co.y, si.y);
+                    turn(a[n].z, b[n].z, co.z, si.z);
+                    turn(a[n].w, b[n].w, co.w, si.w);
+                }
+            }
+            put4(o + d0[n], a[n]);
+            put4(o + d1[n], b[n]);
         }
     }
-    put4(o + d0, a);
-    put4(o + d1, b);
 }
 
 // Any even rotated part: a pair to a thread.
 template <typename T, typename C>
-__global__ void __launch_bounds__(256)
-    rope_pages_any_kernel(tg_params p, const uint32_t *__restrict__ at, const uint32_t *__restrict__ place,
-                          const C *__restrict__ c, const float *__restrict__ cosv, const float *__restrict__ sinv,
-                          T *__restrict__ q, T *__restrict__ k, T *__restrict__ v, uint32_t *err) {
+__global__ void __launch_bounds__(ROPE_THREADS)
+    rope_pages_any_kernel(tg_params p, Divisor page, Divisor row_units, uint32_t block_rows, const uint32_t *__restrict__ at,
+                          const uint32_t *__restrict__ place, const C *__restrict__ c, const float *__restrict__ cosv,
+                          const float *__restrict__ sinv, T *__restrict__ q, T *__restrict__ k, T *__restrict__ v, uint32_t *err) {
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t units = p.head_dim / 2, heads = p.heads + 2 * p.kv_heads, row_units = units * heads;
-    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (uint64_t)p.rows * row_units) return;
-    const uint32_t row = (uint32_t)(i / row_units), in_row = (uint32_t)(i % row_units), head = in_row / units, u = in_row % units;
-    uint32_t pos, to;
-    if (!rope_row(p, at, place, row, pos, to, err)) return;
-    T *o = rope_out(p, row, head, to, q, k, v);
-    if (!o) return;
-    const C *x = c + ((size_t)row * heads + head) * p.head_dim;
-    const bool turned = p.rope && head < p.heads + p.kv_heads && u < p.k / 2;
-    const bool half = turned && !(p.flags & 1);
-    const uint32_t d0 = half ? u : 2 * u, d1 = half ? p.k / 2 + u : 2 * u + 1;
-    float a = to_f32<C>(x[d0]), b = to_f32<C>(x[d1]);
-    if (turned) turn(a, b, __ldg(cosv + (size_t)pos * (p.k / 2) + u), __ldg(sinv + (size_t)pos * (p.k / 2) + u));
-    o[d0] = from_f32<T>(a);
-    o[d1] = from_f32<T>(b);
+    const uint32_t units = p.head_dim / 2, heads = p.heads + 2 * p.kv_heads;
+    const uint32_t row0 = blockIdx.x * block_rows, here = min(block_rows, p.rows - row0) * row_units.d;
+    for (uint32_t i = threadIdx.x; i < here; i += ROPE_THREADS) {
+        const uint32_t in_block = row_units.div(i), row = row0 + in_block, in_row = i - in_block * row_units.d;
+        const uint32_t u = in_row % units, head = in_row / units, pos = at[row], to = place[row];
+        if (!rope_row(p, pos, to, err)) continue;
+        T *o = rope_out(p, page, row, head, to, q, k, v);
+        if (!o) continue;
+        const C *x = c + ((size_t)row * heads + head) * p.head_dim;
+        const bool turned = p.rope && head < p.heads + p.kv_heads && u < p.k / 2;
+        const bool half = turned && !(p.flags & 1);
+        const uint32_t d0 = half ? u : 2 * u, d1 = half ? p.k / 2 + u : 2 * u + 1;
+        float a = to_f32<C>(x[d0]), b = to_f32<C>(x[d1]);
+        if (turned) turn(a, b, __ldg(cosv + (size_t)pos * (p.k / 2) + u), __ldg(sinv + (size_t)pos * (p.k / 2) + u));
+        o[d0] = from_f32<T>(a);
+        o[d1] = from_f32<T>(b);
+    }
 }
 
 // ---- logits_pick -----------------------------------------------------------------------------------
-// A cluster of blocks to a row, each block a run of PICK_SLICE-token slices: the slice's occurrences
-// counted in shared memory (every entry of the row's history is looked at, whole numbers added
-// atomically: no order shows), then its logits streamed through once. The row's greedy choice is
-// joined over the cluster in distributed shared memory. HBM-bound: each logit read and written once.
-constexpr int PICK_THREADS = 512, PICK_SLICE = 4096, PICK_EACH = PICK_SLICE / PICK_THREADS;
-constexpr uint32_t IN_PROMPT = 1u << 31;  // a slice word: the prompt holds the token; below, its generated occurrences
+// A cluster of blocks to a row, every ranks-th tile of PICK_TILE tokens to each (a history holds many low
+// tokens: in ranges the first block had most of the counting). A block marks its touched tokens (in
+// the history or the biases) in a bit map and numbers them by its running bit counts; their occurrences are
+// added, and a token's last bias entry found, atomically on whole numbers, so that no order shows. The
+// touched logits are then done a thread to a token, and the others pass through without a barrier, four
+// or eight to a 16-byte load and store, the first of them on their way since before the counting. The
+// row's greedy choice is joined over the cluster in distributed shared memory. HBM-bound: each logit is
+// read and written once.
+constexpr int PICK_THREADS = 512;
+constexpr uint32_t PICK_TILE = 1024, PICK_AHEAD = 64 * PICK_TILE;
+constexpr uint32_t PICK_RUN = 65536;     // the most tokens whose bits are held at once
+constexpr uint32_t PICK_TOUCHED = 4096;  // the most touched tokens whose words are held at once
+constexpr size_t PICK_SMEM = (PICK_RUN / 32 + 3 * PICK_TOUCHED) * sizeof(uint32_t) + PICK_RUN / 32 * sizeof(uint16_t);
+// A count word: the prompt holds the token; a bias names it; below, its generated occurrences.
+constexpr uint32_t IN_PROMPT = 1u << 31, BIASED = 1u << 30;
 
 struct Best {
     float value;
@@ -266,19 +310,27 @@ TG_DEVICE void better(Best &a, float value, uint32_t token) {
     if (value > a.value || (value == a.value && token < a.token)) a = Best{value, token};
 }
 
-// VEC consecutive logits to one 16-byte load (1: rows that are not 16-byte aligned).
+// VEC consecutive logits to one load: 16 bytes, or one logit for rows that are not 16-byte aligned.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(PICK_THREADS)
+__global__ void __launch_bounds__(PICK_THREADS, 2)
     logits_pick_kernel(tg_params p, const T *logits, const uint32_t *__restrict__ seen,
                        const uint32_t *__restrict__ spans, const float *__restrict__ penalties,
                        const uint32_t *__restrict__ bias_ids, const float *__restrict__ bias,
                        const uint32_t *__restrict__ masks, T *out, uint32_t *__restrict__ pick, uint32_t *err) {
     namespace cg = cooperative_groups;
-    __shared__ __align__(16) uint32_t count[PICK_SLICE], biased[PICK_SLICE];
-    __shared__ Best warp_best[PICK_THREADS / 32], block_best;
+    using Raw = typename std::conditional<VEC == 1, T, typename Vec<T>::Raw>::type;
+    constexpr int EACH = VEC == 1 ? 8 : 4;  // loads of a thread in flight
+    constexpr uint32_t STEP = PICK_THREADS * VEC * EACH, ALL = (1u << VEC) - 1;
+    extern __shared__ __align__(16) uint32_t pick_smem[];
+    uint32_t *touched = pick_smem, *count = touched + PICK_RUN / 32, *biased = count + PICK_TOUCHED;
+    ushort2 *token = reinterpret_cast<ushort2 *>(biased + PICK_TOUCHED);  // touched tokens, and where they are counted
+    uint16_t *before = reinterpret_cast<uint16_t *>(token + PICK_TOUCHED);
+    __shared__ Best warp_best[PICK_THREADS / 32], block_best[8];  // the first block's: of every block
+    __shared__ uint32_t warp_bits[PICK_THREADS / 32], listed;
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t tid = threadIdx.x, ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t row = blockIdx.x / ranks, n = p.n;
+    cluster.sync();  // every block has started before its shared memory is written
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t *span = spans + (size_t)row * 6;
@@ -290,117 +342,209 @@ __global__ void __launch_bounds__(PICK_THREADS)
     }
     const uint32_t history = prompt + made;
     const float repetition = penalties[(size_t)row * 3], presence = penalties[(size_t)row * 3 + 1], frequency = penalties[(size_t)row * 3 + 2];
-    const uint32_t *bits = masks + (size_t)(mask == SPARE ? 0 : mask) * ((n + 31) / 32);
+    const uint32_t *bits = mask == SPARE ? nullptr : masks + (size_t)mask * ((n + 31) / 32);
     const T *x = logits + (size_t)row * p.stride;
     T *y = out + (size_t)row * p.stride;
-    Best best{-INFINITY, SPARE};
-    const uint32_t slices = (n + PICK_SLICE - 1) / PICK_SLICE;
-    for (uint32_t slice = rank; slice < slices; slice += ranks) {
-        const uint32_t t0 = slice * PICK_SLICE;
-        // The slice's logits are on their way while its history is counted.
-        float v[PICK_EACH];
+    Best best{-INFINITY, SPARE}, other{-INFINITY, SPARE};  // of the untouched tokens, and of the touched ones
+    const bool controls = history || biases;
+    const uint32_t rank_bits = 31 - __clz(ranks);  // ranks is a power of two
+    // The block's tokens in ascending order, as numbers l of its own: the token of l, and a token's l (none: past all).
+    const uint32_t tiles = (n + PICK_TILE - 1) / PICK_TILE, mine = tiles > rank ? (tiles - rank + ranks - 1) / ranks * PICK_TILE : 0;
+    auto token_of = [&](uint32_t l) { return (l / PICK_TILE * ranks + rank) * PICK_TILE + l % PICK_TILE; };
+    auto local_of = [&](uint32_t t) {
+        const uint32_t tile = t / PICK_TILE;
+        return t < n && (tile & (ranks - 1)) == rank ? (tile >> rank_bits) * PICK_TILE + t % PICK_TILE : SPARE;
+    };
+    for (uint32_t l0 = 0, end; l0 < mine; l0 = end) {
+        end = min(mine, l0 + PICK_RUN);
+        Raw raw[EACH];
+        auto load = [&](uint32_t at) {
 #pragma unroll
-        for (int j = 0; j < PICK_EACH / VEC; j++) {
-            const uint32_t t = t0 + (j * PICK_THREADS + tid) * VEC;
-            if constexpr (VEC > 1) {
-                if (t + VEC <= n) {
-                    typename Vec<T>::Raw raw = __ldcs(reinterpret_cast<const typename Vec<T>::Raw *>(x + t));
-                    float f[Vec<T>::N];
-                    Vec<T>::unpack(raw, f);
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) v[j * VEC + e] = f[e];
-                    continue;
-                }
+            for (int j = 0; j < EACH; j++) {
+                const uint32_t t = token_of(at + (j * PICK_THREADS + tid) * VEC);
+                if (t + VEC <= n) raw[j] = __ldcs(reinterpret_cast<const Raw *>(x + t));
             }
-#pragma unroll
-            for (int e = 0; e < VEC; e++) v[j * VEC + e] = t + e < n ? to_f32<T>(x[t + e]) : 0.0f;
-        }
-        const bool controls = history || biases;
+        };
+        // With controls to count first, the run's tiles come into L2 meanwhile (register loads would stand before the
+        // history's in the memory pipe).
+        if (!controls) load(l0);
+        else if (VEC > 1)
+            for (uint32_t l = l0 + tid * PICK_TILE; l < min(end, l0 + PICK_AHEAD); l += PICK_THREADS * PICK_TILE)
+                if (token_of(l) + PICK_TILE <= n)
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x + token_of(l)), "n"(PICK_TILE * sizeof(T)) : "memory");
+        auto allow = [&](uint32_t t) { return bits ? __ldg(bits + t / 32) >> (t % 32) : 0xffffffffu; };
+        auto hits = [&](uint32_t in) { return controls ? touched[in / 32] >> (in % 32) & ALL : 0u; };
         if (controls) {
-            __syncthreads();  // the slice before is done with the words
-            for (uint32_t i = tid; i < PICK_SLICE / 4; i += PICK_THREADS) {
-                reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
-                reinterpret_cast<uint4 *>(biased)[i] = make_uint4(0, 0, 0, 0);
-            }
-            __syncthreads();
-            for (uint32_t i = tid; i < history; i += PICK_THREADS) {
-                const uint32_t t = seen[begin + i] - t0;
-                if (t < PICK_SLICE) {
-                    if (i < prompt) atomicOr(count + t, IN_PROMPT);
-                    else atomicAdd(count + t, 1u);
+            auto entries = [&](auto in_history, auto in_biases) {
+                constexpr int H = 8;  // entries of a thread in flight
+                for (uint32_t i0 = tid; i0 < history; i0 += PICK_THREADS * H) {
+                    uint32_t e[H];
+#pragma unroll
+                    for (int h = 0; h < H; h++) e[h] = i0 + h * PICK_THREADS < history ? __ldg(seen + begin + i0 + h * PICK_THREADS) : SPARE;
+#pragma unroll
+                    for (int h = 0; h < H; h++) {
+                        const uint32_t in = local_of(e[h]) - l0;
+                        if (in < end - l0) in_history(in, i0 + h * PICK_THREADS);
+                    }
                 }
+                for (uint32_t i = tid; i < biases; i += PICK_THREADS) {
+                    const uint32_t in = local_of(bias_ids[bias0 + i]) - l0;
+                    if (in < end - l0) in_biases(in, i);
+                }
+            };
+            constexpr uint32_t W = PICK_RUN / 32 / PICK_THREADS;  // words of the bit map to a thread
+            uint32_t total, upto, marks[W];
+            while (true) {
+                __syncthreads();  // the run before is done with the words
+#pragma unroll
+                for (uint32_t i = 0; i < W; i++) touched[tid + i * PICK_THREADS] = 0;
+                __syncthreads();
+                auto touch = [&](uint32_t in, uint32_t) {
+                    if (!(touched[in / 32] >> (in % 32) & 1)) atomicOr(touched + in / 32, 1u << (in % 32));
+                };
+                entries(touch, touch);
+                __syncthreads();
+                uint32_t sum = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < W; i++) {
+                    marks[i] = touched[tid * W + i];
+                    sum += __popc(marks[i]);
+                }
+                upto = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= (uint32_t)o) upto += u;
+                }
+                if (lane == 31) warp_bits[warp] = upto;
+                __syncthreads();
+                total = 0;
+                for (uint32_t w = 0; w < PICK_THREADS / 32; w++) {
+                    if (w < warp) upto += warp_bits[w];
+                    total += warp_bits[w];
+                }
+                upto -= sum;
+                if (total <= PICK_TOUCHED) break;
+                end = l0 + PICK_TOUCHED;  // of so many tokens no more can be touched
             }
-            for (uint32_t i = tid; i < biases; i += PICK_THREADS) {
-                const uint32_t t = bias_ids[bias0 + i] - t0;
-                if (t < PICK_SLICE) atomicMax(biased + t, i + 1);
+#pragma unroll
+            for (uint32_t i = 0; i < W; i++) {
+                before[tid * W + i] = upto;
+                upto += __popc(marks[i]);
             }
+            for (uint32_t i = tid; i < total; i += PICK_THREADS) count[i] = biased[i] = 0;
+            if (tid == 0) listed = 0;
             __syncthreads();
-        }
+            // The entry that finds its token's count zero lists the token.
+            auto add = [&](uint32_t in, uint32_t i, uint32_t first) {
+                const uint32_t at = before[in / 32] + __popc(touched[in / 32] & ((1u << (in % 32)) - 1));
+                const uint32_t old = first == 1 ? atomicAdd(count + at, 1u) : atomicOr(count + at, first);
+                if (first == BIASED) atomicMax(biased + at, i + 1);
+                if (old == 0) token[atomicAdd(&listed, 1u)] = make_ushort2(in, at);
+            };
+            entries([&](uint32_t in, uint32_t i) { add(in, i, i < prompt ? IN_PROMPT : 1u); }, [&](uint32_t in, uint32_t i) { add(in, i, BIASED); });
+            __syncthreads();
+            constexpr int F = 4;  // touched logits of a thread in flight
+            for (uint32_t i0 = tid; i0 < total; i0 += PICK_THREADS * F) {
+                T value[F];
+                uint32_t all[F];
 #pragma unroll
-        for (int j = 0; j < PICK_EACH / VEC; j++) {
-            const uint32_t in = (j * PICK_THREADS + tid) * VEC, t = t0 + in;
-            if (t >= n) break;
-            uint32_t allowed = 0xffffffffu;
-            if (mask != SPARE) allowed = __ldg(bits + t / 32) >> (t % 32);
-            __align__(16) T stored[VEC];
+                for (int k = 0; k < F; k++) {
+                    const uint32_t i = i0 + k * PICK_THREADS;
+                    if (i >= total) continue;
+                    const uint32_t t = token_of(l0 + token[i].x);
+                    value[k] = x[t];
+                    all[k] = allow(t);
+                }
 #pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                float f = v[j * VEC + e];
-                if (controls) {
-                    const uint32_t c = count[in + e], b = biased[in + e];
-                    if (c) {
-                        const float m = (float)(c & ~IN_PROMPT);
+                for (int k = 0; k < F; k++) {
+                    const uint32_t i = i0 + k * PICK_THREADS;
+                    if (i >= total) continue;
+                    const uint32_t t = token_of(l0 + token[i].x), c = count[token[i].y], b = biased[token[i].y], made = c & (BIASED - 1);
+                    float f = to_f32<T>(value[k]);
+                    if (c & ~BIASED) {
                         f = f > 0.0f ? __fdiv_rn(f, repetition) : f * repetition;
-                        f = f - m * frequency;
-                        if (c & ~IN_PROMPT) f = f - presence;
+                        f = f - (float)made * frequency;
+                        if (made) f = f - presence;
                     }
                     if (b) f = f + bias[bias0 + b - 1];
+                    const float stored = to_f32<T>(from_f32<T>(all[k] & 1 ? f : -INFINITY));
+                    biased[token[i].y] = __float_as_uint(stored);  // stored behind the stream
+                    if (stored > -INFINITY) better(other, stored, t);
                 }
-                if (!(allowed >> e & 1)) f = -INFINITY;
-                stored[e] = from_f32<T>(f);
-                // A thread meets its tokens in ascending order: the first of equal values stays.
-                const float s = to_f32<T>(stored[e]);
-                if (t + e < n && s > best.value) best = Best{s, t + e};
             }
-            if (VEC > 1 && t + VEC <= n) {
-                *reinterpret_cast<typename Vec<T>::Raw *>(y + t) = *reinterpret_cast<const typename Vec<T>::Raw *>(stored);
-            } else {
+        }
+        // The stream: logits masked, stored and, untouched ones, compared with the best so far. A thread meets its
+        // tokens in ascending order, so that the first of equal values stays.
+        for (uint32_t at = l0; at < end; at += STEP) {
+            if (at != l0 || controls) load(at);
+#pragma unroll
+            for (int j = 0; j < EACH; j++) {
+                const uint32_t l = at + (j * PICK_THREADS + tid) * VEC, t = token_of(l);
+                if (l >= end || t + VEC > n) break;
+                const uint32_t hit = hits(l - l0), allowed = allow(t) & ALL;
+                __align__(16) T value[VEC];
+                *reinterpret_cast<Raw *>(value) = raw[j];
+                if (allowed != ALL)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) value[e] = allowed >> e & 1 ? value[e] : from_f32<T>(-INFINITY);
+                __stcs(reinterpret_cast<Raw *>(y + t), *reinterpret_cast<const Raw *>(value));
+                if (hit)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) value[e] = hit >> e & 1 ? from_f32<T>(-INFINITY) : value[e];
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
-                    if (t + e < n) y[t + e] = stored[e];
+                    if (to_f32<T>(value[e]) > best.value) best = Best{to_f32<T>(value[e]), t + e};
             }
         }
+        // The row's last tokens, past its whole vectors.
+        if (VEC > 1 && tid < n % VEC) {
+            const uint32_t t = n / VEC * VEC + tid, l = local_of(t);
+            if (l >= l0 && l < end && !(hits(l - l0) & 1)) {
+                const T value = allow(t) & 1 ? x[t] : from_f32<T>(-INFINITY);
+                y[t] = value;
+                if (to_f32<T>(value) > best.value) best = Best{to_f32<T>(value), t};
+            }
+        }
+        if (controls) {
+            __syncthreads();  // the touched tokens' logits over what the stream left there
+            for (uint32_t i = tid; i < listed; i += PICK_THREADS) y[token_of(l0 + token[i].x)] = from_f32<T>(__uint_as_float(biased[token[i].y]));
+        }
     }
+    better(best, other.value, other.token);
+    auto warp_join = [&](Best v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        better(best, __shfl_xor_sync(0xffffffffu, best.value, o), __shfl_xor_sync(0xffffffffu, best.token, o));
-    if ((tid & 31) == 0) warp_best[tid >> 5] = best;
+        for (int o = 16; o > 0; o >>= 1)
+            better(v, __shfl_xor_sync(0xffffffffu, v.value, o), __shfl_xor_sync(0xffffffffu, v.token, o));
+        return v;
+    };
+    best = warp_join(best);
+    if (lane == 0) warp_best[warp] = best;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < PICK_THREADS / 32; w++) better(best, warp_best[w].value, warp_best[w].token);
-        block_best = best;
+    if (warp == 0) {
+        best = warp_join(lane < PICK_THREADS / 32 ? warp_best[lane] : Best{-INFINITY, SPARE});
+        if (lane == 0) *cluster.map_shared_rank(block_best + rank, 0) = best;
     }
     cluster.sync();
-    if (rank == 0 && tid == 0) {
-        for (uint32_t b = 1; b < ranks; b++) {
-            const Best o = *cluster.map_shared_rank(&block_best, b);
-            better(best, o.value, o.token);
-        }
-        pick[row] = best.token;
+    if (rank == 0 && warp == 0) {
+        best = warp_join(lane < ranks ? block_best[lane] : Best{-INFINITY, SPARE});
+        if (lane == 0) pick[row] = best.token;
     }
-    cluster.sync();  // no block ends while its choice is read
 }
 
 template <typename T, int VEC>
 cudaError_t pick_t(const tg_params &p, const void *logits, const uint32_t *seen, const uint32_t *spans, const float *pen,
                    const uint32_t *ids, const float *bias, const uint32_t *masks, void *out, uint32_t *pick, uint32_t *err,
                    cudaStream_t s) {
-    const uint32_t slices = (p.n + PICK_SLICE - 1) / PICK_SLICE;
-    uint32_t ranks = p.rows <= 64 ? 8 : 4;
-    while (ranks > 1 && ranks / 2 >= slices) ranks /= 2;
+    // Blocks of 1024 tokens at least; eight to a row, or four where rows alone fill the device's four blocks an SM.
+    uint32_t ranks = p.rows <= 32 ? 8 : p.rows <= 64 ? 4 : 2;
+    while (ranks > 1 && p.n <= ranks / 2 * PICK_TILE) ranks /= 2;
+    cudaError_t e = with_smem(logits_pick_kernel<T, VEC>, PICK_SMEM);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.rows * ranks);
     cfg.blockDim = dim3(PICK_THREADS);
+    cfg.dynamicSmemBytes = PICK_SMEM;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -418,12 +562,12 @@ template <typename T, typename C>
 cudaError_t rope_t(const tg_params &p, const uint32_t *at, const uint32_t *place, const void *c, const float *cs,
                    const float *sn, void *q, void *k, void *v, uint32_t *err, cudaStream_t s) {
     const bool wide = p.k % 8 == 0;
-    const uint64_t threads = (uint64_t)p.rows * (p.heads + 2 * p.kv_heads) * (p.head_dim / (wide ? 8 : 2));
-    const uint64_t blocks = (threads + 255) / 256;
-    if (blocks > 0x7fffffffu) return cudaErrorNotSupported;
-    const dim3 grid((unsigned)blocks);
+    const uint32_t heads = p.heads + 2 * p.kv_heads, units = wide ? (heads + 1) / 2 * (p.head_dim / 8) : heads * (p.head_dim / 2);
+    const uint32_t block_rows = units >= ROPE_THREADS ? 1 : ROPE_THREADS / units;
+    const dim3 grid((p.rows + block_rows - 1) / block_rows);
     auto run = [&](auto kern) {
-        return launch_pdl(kern, grid, dim3(256), 0, s, p, at, place, (const C *)c, cs, sn, (T *)q, (T *)k, (T *)v, err);
+        return launch_pdl(kern, grid, dim3(ROPE_THREADS), 0, s, p, Divisor(p.capacity), Divisor(units), block_rows, at, place,
+                          (const C *)c, cs, sn, (T *)q, (T *)k, (T *)v, err);
     };
     if (!wide) return run(rope_pages_any_kernel<T, C>);
     return p.flags & 1 ? run(rope_pages_kernel<T, C, true>) : run(rope_pages_kernel<T, C, false>);
