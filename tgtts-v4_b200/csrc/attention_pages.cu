@@ -9,6 +9,8 @@
 // heads of one KV head, are the 128 rows of its products, so that a tile of keys and values is read
 // once for 128 queries. The own pieces, which no other row shares, run on mma.sync
 // (own_kernel), bound by the caches' bytes. f32 runs on the CUDA cores (pieces_kernel).
+#include <algorithm>
+
 #include "mma_common.cuh"
 #include "tc_common.cuh"
 
@@ -20,7 +22,7 @@ constexpr uint32_t SPARE = TG_SPARE;
 constexpr int CHUNK = 128;  // positions a block takes at once
 
 // Own positions of a piece.
-__host__ __device__ constexpr uint32_t own_piece(uint32_t hd) { return 16384 / hd; }
+constexpr uint32_t OWN_PIECE = 128;
 // Shared positions of a piece: at most 16 pieces, each whole chunks.
 __host__ __device__ inline uint32_t shared_piece(uint32_t first) {
     const uint32_t even = (first + 15) / 16;
@@ -28,7 +30,7 @@ __host__ __device__ inline uint32_t shared_piece(uint32_t first) {
 }
 __host__ __device__ inline uint32_t shared_pieces(uint32_t first) { return (first + shared_piece(first) - 1) / shared_piece(first); }
 __host__ __device__ inline uint64_t all_pieces(const tg_params &p) {
-    return shared_pieces(p.first) + ((uint64_t)p.stride * p.capacity + own_piece(p.head_dim) - 1) / own_piece(p.head_dim);
+    return shared_pieces(p.first) + ((uint64_t)p.stride * p.capacity + OWN_PIECE - 1) / OWN_PIECE;
 }
 
 // The partials in the work buffer, from its first 256-byte boundary: o f32 [rows][heads][pieces][hd], then
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(CHUNK)
     uint32_t length, seq;
     if (!paged_row(p, at, row, length, seq, kv == 0 && piece == 0 && tid == 0 ? err : nullptr)) return;
     const bool own = piece >= (int)np;
-    const uint32_t size = own ? own_piece(HD) : shared_piece(p.first), n = own ? length : p.first;
+    const uint32_t size = own ? OWN_PIECE : shared_piece(p.first), n = own ? length : p.first;
     const uint64_t begin = (uint64_t)(own ? piece - np : piece) * size;
     if (begin >= n) return;
     const uint32_t stop = (uint32_t)min((uint64_t)n, begin + size);
@@ -165,166 +167,280 @@ __global__ void __launch_bounds__(CHUNK)
 }
 
 // ---- own pieces, bf16 ---------------------------------------------------------------------------------
-// A block to a piece of a row's own positions for one KV head, a quarter of it to each of four warps:
-// the group's query heads are the rows of mma.sync.m16n8k16 (S = q K^T, O = e V with e split into bf16
-// hi + lo), keys and values gathered from their pages into the warp's shared memory by cp.async, all in
-// flight at once. The block joins its warps' partials in shared memory. References are in base 2.
-constexpr int OWN_WARPS = 4;
-constexpr int own_row(int hd) { return hd + fa::PAD; }  // bf16 of a shared row
-constexpr int own_smem(int hd) { return 2 * (int)own_piece(hd) * own_row(hd) * 2; }
+// A warp to a piece of a row's own positions for one KV head, in chunks of own_chunk positions: the group's
+// query heads, at most 8, are the columns of mma.sync.m16n8k16 (S^T = K q^T, O^T = V^T e^T with e split
+// into bf16 hi + lo, against a reference that moves as prefix_kernel's), keys and values brought by TMA, 16
+// positions of one page and 64 dimensions to a copy, two chunks ahead of the products. Bound by the caches'
+// bytes at the rate that the warps' chains of products and exponentials let through: eight warps an SM that
+// share nothing. (Gathered by cp.async, 16 copies and 16 shuffles a lane and chunk, six warps took 35 us for
+// 134 MB, 64 rows of 32 heads of 128.) Blocks take their pieces off a list of the live ones alone, which each
+// makes from the rows' lengths by a scan. References are in base 2.
+constexpr int OWN_STAGES = 3;
+constexpr uint32_t OWN_ROWS = 192;  // rows whose pieces are listed at once
+constexpr int own_chunk(int hd) { return 2048 / hd; }
+constexpr uint32_t OWN_BOX = 16 * 128;            // a copy: 16 positions of 64 dimensions
+constexpr uint32_t OWN_TILE = 4 * 1024;           // a chunk's keys, or values, by boxes
+constexpr int OWN_SMEM = OWN_STAGES * 2 * (int)OWN_TILE + 1024 + (int)OWN_ROWS * 12;
+constexpr int OWN_BLOCKS = 8;  // an SM's, by their shared memory
+
+// An 8 x 8 block of 16-bit values over a warp (lane 4 r + c: columns 2 c and 2 c + 1 of row r), transposed.
+TG_DEVICE uint32_t turn8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// How far (base 2) a maximum may pass a query's reference before O and l are rescaled.
+constexpr float MOVE_PAST = 8.0f;
 
 template <int HD>
-__global__ void __launch_bounds__(OWN_WARPS * 32)
-    own_kernel(tg_params p, const bf16 *__restrict__ q, const bf16 *__restrict__ k, const bf16 *__restrict__ v,
-               const uint32_t *__restrict__ at, const uint32_t *__restrict__ table, Partials out, uint32_t np,
-               uint32_t pieces, uint32_t *err) {
+__global__ void __launch_bounds__(32)
+    own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, tg_params p,
+               const bf16 *__restrict__ q, const uint32_t *__restrict__ at, const uint32_t *__restrict__ table, Partials out,
+               uint32_t np, uint32_t pieces, uint32_t *err) {
     using namespace fa;
-    extern __shared__ __align__(128) unsigned char own_mem[];
-    constexpr int W = own_piece(HD) / OWN_WARPS, ROW = own_row(HD), NT = W / 8, DT = HD / 8, VECS = HD / 8;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ __align__(8) uint64_t full[OWN_STAGES];
+    __shared__ int gave_up;
+    constexpr int CH = own_chunk(HD), HALVES = HD / 64, G16 = CH / 16;
+    const uint32_t lane = threadIdx.x, g = lane >> 2, t4 = lane & 3, mi = lane >> 3, rr = lane & 7;
+    if (lane == 0) {
+        gave_up = 0;
+        for (int i = 0; i < OWN_STAGES; i++) mbar_init(smem_u32(full + i), 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
     // Behind prefix_kernel this one starts under it: that kernel lets it go once what comes before both has
     // ended (its own wait), and the two share nothing. A block still waits before it ends, for the join.
     if (np == 0) pdl_wait();
     pdl_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int kv = blockIdx.y, row = blockIdx.z, heads = p.heads, kvh = p.kv_heads, group = heads / kvh;
-    uint32_t length, seq;
-    if (!paged_row(p, at, row, length, seq, kv == 0 && blockIdx.x == 0 && threadIdx.x == 0 ? err : nullptr) ||
-        (uint64_t)blockIdx.x * own_piece(HD) >= length) {
-        pdl_wait();
-        return;
-    }
-    bf16 *ks = reinterpret_cast<bf16 *>(own_mem) + (size_t)warp * 2 * W * ROW, *vs = ks + W * ROW;
-    const uint32_t start = blockIdx.x * own_piece(HD) + warp * W;
-    const int live = start < length ? (int)min(length - start, (uint32_t)W) : 0;  // positions of this warp
-    float m = -INFINITY, l = 0.0f, o[DT][4];
+    const int heads = p.heads, kvh = p.kv_heads, group = heads / kvh;
+    // The rows of a list: the pieces before each, its own length and its request.
+    uint32_t *first_piece = reinterpret_cast<uint32_t *>(smem + OWN_STAGES * 2 * OWN_TILE), *lengths = first_piece + OWN_ROWS,
+             *requests = lengths + OWN_ROWS;
+    const float scale2 = 1.4426950408889634f / sqrtf((float)HD);
+    uint32_t used = 0, issued = 0;  // chunks of the pieces done, and issued: stages and their barriers' phases
+    for (uint32_t row0 = 0; row0 < p.rows; row0 += OWN_ROWS) {
+        const uint32_t rows = min(OWN_ROWS, p.rows - row0);
+        uint32_t total = 0;
+        __syncwarp();
+        for (uint32_t r0 = 0; r0 < rows; r0 += 32) {
+            const uint32_t r = r0 + lane;
+            uint32_t length = 0, seq = 0;
+            if (r >= rows || !paged_row(p, at, row0 + r, length, seq, blockIdx.x == 0 ? err : nullptr)) length = 0;
+            const uint32_t n = (length + OWN_PIECE - 1) / OWN_PIECE;
+            uint32_t upto = n;
 #pragma unroll
-    for (int j = 0; j < DT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-    if (live) {
-        uint64_t from[W / 32];  // where positions lane, lane + 32, .. lie in the caches
-#pragma unroll
-        for (int i = 0; i < W / 32; i++) {
-            const uint32_t pos = start + min(lane + 32 * i, live - 1);
-            uint32_t id = __ldg(table + (size_t)seq * p.stride + pos / p.capacity);
-            if (id >= p.slots) {
-                atomicExch(err, ERR_BAD_INDEX);
-                id = 0;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= (uint32_t)o) upto += u;
             }
-            from[i] = (((uint64_t)id * kvh + kv) * p.capacity + pos % p.capacity) * HD;
+            if (r < rows) {
+                first_piece[r] = total + upto - n;
+                lengths[r] = length;
+                requests[r] = seq;
+            }
+            total += __shfl_sync(0xffffffffu, upto, 31);
         }
-        auto gather = [&](bf16 *to, const bf16 *cache) {
-#pragma unroll
-            for (int i = 0; i < W * VECS / 32; i++) {
-                const int r = i * (32 / VECS) + lane / VECS, c = lane % VECS;
-                uint64_t src = __shfl_sync(0xffffffffu, from[(i * (32 / VECS)) / 32], r % 32);
-                cp_async16(to + r * ROW + c * 8, cache + src + c * 8, r < live);
-            }
-            cp_async_commit();
+        __syncwarp();
+        // A piece: its row, number, KV head, live positions and their chunks (0: none); lane i < 8 the page's number and
+        // the offset in it of positions begin + 16 i .. . It is looked up a piece ahead of its copies.
+        struct Piece {
+            uint32_t row, number, page, offset;
+            int kv, live, chunks;
         };
-        gather(ks, k);
-        gather(vs, v);
-        // q of the group's heads: rows g < group of the products (rows past it, and 8 to 15, zero).
-        uint32_t qf[HD / 16][4];
-        const bf16 *qg = q + ((size_t)row * heads + kv * group + g) * HD + 2 * t4;
-#pragma unroll
-        for (int s = 0; s < HD / 16; s++) {
-            qf[s][0] = g < group ? __ldg(reinterpret_cast<const uint32_t *>(qg + 16 * s)) : 0u;
-            qf[s][2] = g < group ? __ldg(reinterpret_cast<const uint32_t *>(qg + 16 * s + 8)) : 0u;
-            qf[s][1] = qf[s][3] = 0u;
-        }
-        cp_async_wait<1>();
-        __syncwarp();
-        const int mi = lane >> 3, rr = lane & 7;
-        float sc[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; j++) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < HD / 16; s++)
-#pragma unroll
-            for (int j = 0; j < NT; j += 2) {
-                uint32_t kb[4];
-                ldmatrix_x4(kb, ks + (8 * j + (mi >> 1) * 8 + rr) * ROW + s * 16 + (mi & 1) * 8);
-                mma_bf16(sc[j], qf[s], kb[0], kb[1]);
-                mma_bf16(sc[j + 1], qf[s], kb[2], kb[3]);
+        const uint64_t tasks = (uint64_t)total * kvh;
+        auto find = [&](uint64_t task) {
+            Piece x{};
+            if (task >= tasks) return x;
+            const uint32_t u = (uint32_t)(task / kvh);
+            uint32_t lo = 0, hi = rows;  // the row with first_piece at most u, its next above
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (first_piece[mid] <= u) lo = mid;
+                else hi = mid;
             }
-        const float scale2 = 1.4426950408889634f / sqrtf((float)HD);
+            x.row = row0 + lo;
+            x.number = u - first_piece[lo];
+            x.kv = (int)(task % kvh);
+            const uint32_t begin = x.number * OWN_PIECE;
+            x.live = (int)min(lengths[lo] - begin, OWN_PIECE);
+            x.chunks = (x.live + CH - 1) / CH;
+            const uint32_t pos = begin + min(16 * (lane & 7), (uint32_t)(x.live - 1) & ~15u);
+            x.page = __ldg(table + (size_t)requests[lo] * p.stride + pos / p.capacity);
+            x.offset = pos % p.capacity;
+            return x;
+        };
+        // Chunk c of a piece into stage `slot` % OWN_STAGES: boxes [16 positions of the chunk][half], each 16 swizzled rows
+        // of 128 bytes.
+        auto fetch = [&](const Piece &x, int c, uint32_t slot) {
+            const uint32_t stage = slot % OWN_STAGES, bar = smem_u32(full + stage), to = smem_u32(smem) + stage * 2 * OWN_TILE;
+            const int boxes = min(G16, (x.live - c * CH + 15) / 16);
+            if (lane == 0) mbar_arrive_expect_tx(bar, 2 * HALVES * boxes * OWN_BOX);
 #pragma unroll
-        for (int j = 0; j < NT; j++)
+            for (int i = 0; i < G16; i++) {
+                uint32_t id = __shfl_sync(0xffffffffu, x.page, c * G16 + i);
+                const int y = (int)__shfl_sync(0xffffffffu, x.offset, c * G16 + i);
+                if (lane == 0 && i < boxes) {
+                    if (id >= p.slots) {
+                        atomicExch(err, ERR_BAD_INDEX);
+                        id = 0;
+                    }
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++) {
+                        tma_load_3d(to + (i * HALVES + h) * OWN_BOX, &kmap, 64 * h, y, (int)(id * kvh + x.kv), bar);
+                        tma_load_3d(to + OWN_TILE + (i * HALVES + h) * OWN_BOX, &vmap, 64 * h, y, (int)(id * kvh + x.kv), bar);
+                    }
+                }
+            }
+        };
+        uint64_t task = blockIdx.x;
+        Piece cur = find(task), next = find(task + gridDim.x);
+        // Issues the chunks before the `upto`-th, of the current piece and, behind its last, the next one (none further:
+        // what a short next piece leaves room for is issued once it is the current one).
+        auto fetch_upto = [&](uint32_t upto) {
+            while (issued < upto) {
+                const int c = (int)(issued - used);
+                if (c < cur.chunks) fetch(cur, c, issued);
+                else if (c - cur.chunks < next.chunks) fetch(next, c - cur.chunks, issued);
+                else break;
+                issued++;
+            }
+        };
+        fetch_upto(used + OWN_STAGES - 1);
+        while (cur.chunks) {
+            const uint32_t row = cur.row;
+            const int kv = cur.kv, live = cur.live, chunks = cur.chunks;
+            // q of the group's heads as columns g < group of the products (those past it zero).
+            uint32_t qf[HD / 16][2];
+            const bf16 *qg = q + ((size_t)row * heads + kv * group + g) * HD + 2 * t4;
+#pragma unroll
+            for (int s = 0; s < HD / 16; s++) {
+                qf[s][0] = (int)g < group ? __ldg(reinterpret_cast<const uint32_t *>(qg + 16 * s)) : 0u;
+                qf[s][1] = (int)g < group ? __ldg(reinterpret_cast<const uint32_t *>(qg + 16 * s + 8)) : 0u;
+            }
+            // A lane's heads 2 t4 and 2 t4 + 1: references, sums, and dimensions g and g + 8 of each 16 of O^T.
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[HD / 16][4];
+#pragma unroll
+            for (int j = 0; j < HD / 16; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+            for (int c = 0; c < chunks; c++) {
+                const uint32_t stage = (used + c) % OWN_STAGES;
+                __syncwarp();  // every lane is done with the chunk before, whose stage is the next to be filled
+                fetch_upto(used + c + OWN_STAGES);
+                mbar_wait(smem_u32(full + stage), ((used + c) / OWN_STAGES) & 1, err, &gave_up);
+                uint8_t *ks = smem + stage * 2 * OWN_TILE, *vs = ks + OWN_TILE;
+                // 16 bytes `part` (of 8 dimensions) of position r of the chunk.
+                auto spot = [](uint8_t *tile, int r, int part) {
+                    return tile + ((r / 16) * HALVES + part / 8) * OWN_BOX + (r % 16) * 128 + ((part % 8 ^ (r & 7)) << 4);
+                };
+                if (live - c * CH < CH) {  // values past the row's length may be anything: 0 x NaN is NaN
+                    for (int i = lane; i < (CH - (live - c * CH)) * (HD / 8); i += 32)
+                        *reinterpret_cast<uint4 *>(spot(vs, live - c * CH + i / (HD / 8), i % (HD / 8))) = make_uint4(0u, 0u, 0u, 0u);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before a later copy into the stage
+                    __syncwarp();
+                }
+                float sc[G16][4];  // positions g and g + 8 of each 16, the lane's two heads
+#pragma unroll
+                for (int j = 0; j < G16; j++) {
+                    float odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // two sums, for two chains of products
+                    sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < HD / 16; s++) {
+                        uint32_t ka[4];
+                        ldmatrix_x4(ka, spot(ks, 16 * j + (mi & 1) * 8 + rr, 2 * s + (mi >> 1)));
+                        mma_bf16(s & 1 ? odd : sc[j], ka, qf[s][0], qf[s][1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float v = (sc[j][e] + odd[e]) * scale2;
+                        sc[j][e] = c * CH + 16 * j + (int)g + 8 * (e >> 1) < live ? v : -INFINITY;
+                    }
+                }
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < G16; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx[e & 1] = fmaxf(mx[e & 1], sc[j][e]);
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) {
+                    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], x));
+                    mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], x));
+                }
+                const bool move[2] = {mx[0] > m[0] + MOVE_PAST, mx[1] > m[1] + MOVE_PAST};
+                if (__any_sync(0xffffffffu, move[0] || move[1])) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        if (!move[e]) continue;
+                        const float keep = m[e] == -INFINITY ? 0.0f : exp2f(m[e] - mx[e]);
+                        m[e] = mx[e];
+                        l[e] *= keep;
+#pragma unroll
+                        for (int j = 0; j < HD / 16; j++) {
+                            o[j][e] *= keep;
+                            o[j][2 + e] *= keep;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < G16; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        sc[j][e] = sc[j][e] == -INFINITY ? 0.0f : exp2f(sc[j][e] - m[e & 1]);
+                        l[e & 1] += sc[j][e];  // the lane's positions' alone
+                    }
+#pragma unroll
+                for (int s = 0; s < G16; s++) {
+                    // e^T as the second operand: each 8 x 8 block turned over among the lanes.
+                    uint32_t h0, h1, l0, l1;
+                    split_pack(sc[s][0], sc[s][1], h0, l0);
+                    split_pack(sc[s][2], sc[s][3], h1, l1);
+                    h0 = turn8(h0);
+                    h1 = turn8(h1);
+                    l0 = turn8(l0);
+                    l1 = turn8(l1);
+#pragma unroll
+                    for (int j = 0; j < HD / 16; j++) {
+                        uint32_t va[4];
+                        ldmatrix_x4_trans(va, spot(vs, 16 * s + (mi >> 1) * 8 + rr, 2 * j + (mi & 1)));
+                        mma_bf16(o[j], va, h0, h1);
+                        mma_bf16(o[j], va, l0, l1);
+                    }
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                sc[j][e] = 8 * j + 2 * t4 + e < live ? sc[j][e] * scale2 : -INFINITY;
-                m = fmaxf(m, sc[j][e]);
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+                const int head = 2 * t4 + e;
+                if (head >= group) continue;
+                const size_t to = ((size_t)row * heads + kv * group + head) * pieces + np + cur.number;
+#pragma unroll
+                for (int j = 0; j < HD / 16; j++) {
+                    out.o[to * HD + 16 * j + g] = o[j][e];
+                    out.o[to * HD + 16 * j + 8 + g] = o[j][2 + e];
+                }
+                if (g == 0) *reinterpret_cast<float2 *>(out.ml + to * 2) = make_float2(m[e], l[e]);
             }
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                sc[j][e] = sc[j][e] == -INFINITY ? 0.0f : exp2f(sc[j][e] - m);
-                l += sc[j][e];
-            }
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        cp_async_wait<0>();
-        __syncwarp();
-#pragma unroll
-        for (int s = 0; s < W / 16; s++) {
-            uint32_t ph[4], pl[4];
-            split_pack(sc[2 * s][0], sc[2 * s][1], ph[0], pl[0]);
-            split_pack(sc[2 * s + 1][0], sc[2 * s + 1][1], ph[2], pl[2]);
-            ph[1] = ph[3] = pl[1] = pl[3] = 0u;
-#pragma unroll
-            for (int j = 0; j < DT; j += 2) {
-                uint32_t vb[4];
-                ldmatrix_x4_trans(vb, vs + (16 * s + (mi & 1) * 8 + rr) * ROW + 8 * j + (mi >> 1) * 8);
-                mma_bf16(o[j], ph, vb[0], vb[1]);
-                mma_bf16(o[j], pl, vb[0], vb[1]);
-                mma_bf16(o[j + 1], ph, vb[2], vb[3]);
-                mma_bf16(o[j + 1], pl, vb[2], vb[3]);
-            }
+            used += chunks;
+            cur = next;
+            task += gridDim.x;
+            next = find(task + gridDim.x);
         }
-    }
-    // The warps' partials joined in warp order (a warp past the row's length: m -inf, o zero).
-    constexpr int G = MAX_GROUP;
-    float *red = reinterpret_cast<float *>(own_mem);  // [OWN_WARPS][G][HD], then [OWN_WARPS][G][2]
-    float *red_ml = red + OWN_WARPS * G * HD;
-    __syncthreads();  // every warp is done with its keys and values
-    if (g < group) {
-        float *dst = red + (warp * G + g) * HD + 2 * t4;
-#pragma unroll
-        for (int j = 0; j < DT; j++) *reinterpret_cast<float2 *>(dst + 8 * j) = make_float2(o[j][0], o[j][1]);
-        if (t4 == 0) *reinterpret_cast<float2 *>(red_ml + (warp * G + g) * 2) = make_float2(m, l);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < group * (HD / 4); i += OWN_WARPS * 32) {
-        const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
-        float mx = -INFINITY, sum = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < OWN_WARPS; w++) mx = fmaxf(mx, red_ml[(w * G + h) * 2]);
-#pragma unroll
-        for (int w = 0; w < OWN_WARPS; w++) {
-            const float mw = red_ml[(w * G + h) * 2], e = mw == -INFINITY ? 0.0f : exp2f(mw - mx);
-            const float4 x = *reinterpret_cast<const float4 *>(red + (w * G + h) * HD + d);
-            sum = __fmaf_rn(red_ml[(w * G + h) * 2 + 1], e, sum);
-            acc = make_float4(__fmaf_rn(x.x, e, acc.x), __fmaf_rn(x.y, e, acc.y), __fmaf_rn(x.z, e, acc.z), __fmaf_rn(x.w, e, acc.w));
-        }
-        const size_t to = ((size_t)row * heads + kv * group + h) * pieces + np + blockIdx.x;
-        *reinterpret_cast<float4 *>(out.o + to * HD + d) = acc;
-        if (d == 0) *reinterpret_cast<float2 *>(out.ml + to * 2) = make_float2(mx, sum);
     }
     pdl_wait();
 }
 
 // ---- shared pieces, bf16 ------------------------------------------------------------------------------
-// Block (piece, t, kv): NT tiles of up to 128 queries, query m of a tile being head m % group of row
-// m / group of the tile's rows, against the piece's keys in tiles of 128. Ten warps (six for one tile):
-//   warp 0     TMA: Q, then K and V tiles page by page (boxes of the largest of 128, 64, 32 and 16
-//              positions that divides a page) into STAGES stages of 128-byte-swizzled halves of 64
-//              dimensions; values past the prefix in its last tile set to zero (0 x NaN is NaN);
+// A block an SM, over units of a piece, a KV head and NT tiles of up to 128 queries, query m of a tile being
+// head m % group of row m / group of the tile's rows, against the piece's keys in tiles of 128. Eleven warps (seven for one tile):
+//   warps 0 and the last  TMA: Q and the K tiles, and the V tiles, page by page (boxes of the largest of
+//              128, 64, 32 and 16 positions that divides a page) into STAGES stages of
+//              128-byte-swizzled halves of 64 dimensions; values past the prefix in its last tile set to
+//              zero (0 x NaN is NaN). Two warps, as a copy's issue takes about 110 clocks: 16 to a tile
+//              of K or V for pages of 16 (8 KiB of HD = 128 each);
 //   warp 1     TMEM and the MMAs: S_j = Q K_j^T (M = 128, N = 128), O += P_j V_j (N = HD; P in TMEM, V
 //              read MN-major), the tile's next S ahead of its PV so that the softmax runs under it;
-//   warps 2-5  (and 6-9) the softmax of a tile, a thread to a query: P_j = 2^(S_j scale - mref) as bf16
+//   warps 2-5  (and 6-9)  the softmax of a tile, a thread to a query: P_j = 2^(S_j scale - mref) as bf16
 //              into TMEM against a reference that moves only when a tile's maximum passes it by 2^8 (O
 //              then rescaled in place), the same pass as the prefill's attention kernel.
 // HD = 64: two tiles, which share the keys' copies, each with S, P and O in 256 columns. HD = 128: one tile
@@ -333,16 +449,13 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
 template <int HD>
 struct Pfx {
     static constexpr int NT = HD == 64 ? 2 : 1, HALVES = HD / 64, STAGES = HD == 64 ? 3 : 2;
-    static constexpr int THREADS = 64 + 128 * NT, SB = HD == 64 ? 1 : 2;
+    static constexpr int THREADS = 96 + 128 * NT, SB = HD == 64 ? 1 : 2;
     static constexpr uint32_t HALF = 128 * 64 * 2, TILE = HALF * HALVES;  // 128 rows x 64 dimensions; x HD
     static constexpr uint32_t Q = 0, K = NT * TILE, V = K + STAGES * TILE, SMEM = V + STAGES * TILE + 1024;
     static constexpr TG_DEVICE uint32_t s_col(int h, int j) { return NT == 2 ? 256 * h : 128 * (j & 1); }
     static constexpr TG_DEVICE uint32_t p_col(int h) { return NT == 2 ? 256 * h + 128 : 256; }
     static constexpr TG_DEVICE uint32_t o_col(int h) { return NT == 2 ? 256 * h + 192 : 320; }
 };
-// How far (base 2) a tile's maximum may pass a query's reference before O and l are rescaled.
-constexpr float MOVE_PAST = 8.0f;
-
 // 2^x by the hardware's base-2 exponential (relative error about 2^-22); 2^-inf = 0.
 TG_DEVICE float hw_exp2(float x) {
     float y;
@@ -377,13 +490,6 @@ TG_DEVICE uint64_t mn_desc(uint32_t addr, uint32_t chunk) {
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-// 32 aligned bytes in one store: a whole sector.
-TG_DEVICE void store8(float *dst, const uint32_t *v) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
-                 "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
-
 template <int HD>
 __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
     prefix_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -393,23 +499,21 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t base = smem_u32(smem);
-    __shared__ __align__(8) uint64_t bq, bk_full[C::STAGES], bk_empty[C::STAGES], bv_full[C::STAGES], bv_empty[C::STAGES];
+    __shared__ __align__(8) uint64_t bq_full, bq_empty, bk_full[C::STAGES], bk_empty[C::STAGES], bv_full[C::STAGES], bv_empty[C::STAGES];
     __shared__ __align__(8) uint64_t bs_full[C::NT * C::SB], bp_full[C::NT], bo_full[C::NT], bv_clear;
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
-    const int kv = blockIdx.z, heads = p.heads, kvh = p.kv_heads, group = heads / kvh;
-    const int tile_rows = 128 / group, tiles = ((int)p.rows + tile_rows - 1) / tile_rows;
-    const int tile0 = blockIdx.y * C::NT, nt = min(C::NT, tiles - tile0);
-    const uint32_t begin = blockIdx.x * shared_piece(p.first), keys = min(shared_piece(p.first), p.first - begin);
-    const int n = (int)((keys + 127) / 128);
-    const bool clear_v = keys % 128 != 0;
+    const int heads = p.heads, kvh = p.kv_heads, group = heads / kvh, tile_rows = 128 / group;
+    const int tiles = ((int)p.rows + tile_rows - 1) / tile_rows, pairs = (tiles + C::NT - 1) / C::NT;
+    const uint32_t size = shared_piece(p.first), np = shared_pieces(p.first), units = np * pairs * kvh;
     auto B = [](uint64_t &b) { return smem_u32(&b); };
 
     if (tid == 0) {
         gave_up = 0;
-        mbar_init(B(bq), 1);
+        mbar_init(B(bq_full), 1);
+        mbar_init(B(bq_empty), 4 * C::NT);
         for (int i = 0; i < C::STAGES; i++) {
             mbar_init(B(bk_full[i]), 1);
             mbar_init(B(bk_empty[i]), 1);
@@ -425,10 +529,13 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // The rows of a Q tile that no query fills (a group that does not divide 128) are zero.
-    for (int i = tid; i < C::NT * C::HALVES * (128 - tile_rows * group) * 8; i += C::THREADS) {
-        const int part = i / ((128 - tile_rows * group) * 8), r = tile_rows * group + i / 8 % (128 - tile_rows * group);
-        *reinterpret_cast<uint4 *>(smem + C::Q + part * C::HALF + r * 128 + (i % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
-    }
+    const int blank = 128 - tile_rows * group;
+    auto blank_q = [&](int h, int i0, int step) {
+        for (int i = i0; i < C::HALVES * blank * 8; i += step)
+            *reinterpret_cast<uint4 *>(smem + C::Q + h * C::TILE + i / (blank * 8) * C::HALF + (tile_rows * group + i / 8 % blank) * 128 + (i % 8) * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
+    };
+    for (int h = 0; h < C::NT; h++) blank_q(h, tid, C::THREADS);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
@@ -443,226 +550,284 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
     pdl_wait();
     pdl_launch_dependents();
 
-    if (warp == 0) {
-        if (lane == 0) {
-            mbar_arrive_expect_tx(B(bq), nt * C::HALVES * tile_rows * group * 128);
-            for (int h = 0; h < nt; h++)
-                for (int c = 0; c < C::HALVES; c++)
-                    tma_load_3d(base + C::Q + h * C::TILE + c * C::HALF, &qmap, c * 64, kv * group, (tile0 + h) * tile_rows, B(bq));
-        }
-        // A lane to a copy: one half of the dimensions, one box of positions. Keys run a tile ahead of
-        // values, as their stages come free earlier, and the pages' numbers a tile ahead of the keys.
+    // A unit: a piece of the prefix, a KV head, NT tiles of queries. The roles walk the block's units each by itself;
+    // `t` counts the tiles of keys over all of them (stages, and their barriers' phases).
+    struct Unit {
+        uint32_t piece, begin, keys;
+        int kv, tile0, nt, n;
+    };
+    auto unit = [&](uint32_t u) {
+        Unit x;
+        x.piece = u % np;
+        x.tile0 = (int)(u / np % pairs) * C::NT;
+        x.kv = (int)(u / np / pairs);
+        x.nt = min(C::NT, tiles - x.tile0);
+        x.begin = x.piece * size;
+        x.keys = min(size, p.first - x.begin);
+        x.n = (int)((x.keys + 127) / 128);
+        return x;
+    };
+    const bool values = warp == C::THREADS / 32 - 1;
+    if (warp == 0 || values) {
+        // A lane to a copy: one half of the dimensions, one box of positions; the pages' numbers a tile ahead.
         const int boxes = 128 / (int)box, seg = lane % boxes, half = lane / boxes;
-        auto page_of = [&](int j) {
-            const uint32_t in = j * 128 + seg * box;
-            uint32_t id = in < keys ? __ldg(shared + (begin + in) / p.capacity) : 0u;
-            if (id >= p.slots) {
-                atomicExch(err, ERR_BAD_INDEX);
-                id = 0;
+        uint64_t *full = values ? bv_full : bk_full, *empty = values ? bv_empty : bk_empty;
+        const CUtensorMap *map = values ? &vmap : &kmap;
+        int t = 0, done = 0, last_clear = -1;  // last_clear: the tile whose values were last cleared
+        for (uint32_t u = blockIdx.x; u < units; u += gridDim.x, done++) {
+            const Unit x = unit(u);
+            auto page_of = [&](int j) {
+                const uint32_t in = j * 128 + seg * box;
+                uint32_t id = in < x.keys ? __ldg(shared + (x.begin + in) / p.capacity) : 0u;
+                if (id >= p.slots) {
+                    atomicExch(err, ERR_BAD_INDEX);
+                    id = 0;
+                }
+                return id;
+            };
+            uint32_t id = page_of(0);
+            for (int j = 0; j < x.n; j++, t++) {
+                const int b = t % C::STAGES, live = min(128, (int)x.keys - j * 128), segs = (live + (int)box - 1) / (int)box;
+                const uint32_t pos = x.begin + j * 128 + seg * box, next = page_of(j + 1);
+                mbar_wait(B(empty[b]), ((t / C::STAGES) & 1) ^ 1, err, &gave_up);
+                if (lane == 0) mbar_arrive_expect_tx(B(full[b]), C::HALVES * segs * box * 128);
+                __syncwarp();
+                if (half < C::HALVES && seg < segs)
+                    tma_load_3d(base + (values ? C::V : C::K) + b * C::TILE + half * C::HALF + seg * box * 128, map, half * 64,
+                                (int)(pos % p.capacity), (int)(id * kvh + x.kv), B(full[b]));
+                id = next;
+                if (warp == 0 && j == 0) {
+                    // Q, once the unit before is done with its own (and with what it staged there).
+                    mbar_wait(B(bq_empty), (done & 1) ^ 1, err, &gave_up);
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(B(bq_full), x.nt * C::HALVES * tile_rows * group * 128);
+                        for (int h = 0; h < x.nt; h++)
+                            for (int c = 0; c < C::HALVES; c++)
+                                tma_load_3d(base + C::Q + h * C::TILE + c * C::HALF, &qmap, c * 64, x.kv * group, (x.tile0 + h) * tile_rows, B(bq_full));
+                    }
+                    __syncwarp();
+                }
             }
-            return id;
-        };
-        auto load = [&](int j, uint32_t id, uint32_t dst, const CUtensorMap *map, uint64_t *full, uint64_t *empty) {
-            const int b = j % C::STAGES, live = min(128, (int)keys - j * 128), segs = (live + (int)box - 1) / (int)box;
-            const uint32_t pos = begin + j * 128 + seg * box;
-            mbar_wait(B(empty[b]), ((j / C::STAGES) & 1) ^ 1, err, &gave_up);
-            if (lane == 0) mbar_arrive_expect_tx(B(full[b]), C::HALVES * segs * box * 128);
-            __syncwarp();
-            if (half < C::HALVES && seg < segs)
-                tma_load_3d(base + dst + b * C::TILE + half * C::HALF + seg * box * 128, map, half * 64, (int)(pos % p.capacity),
-                            (int)(id * kvh + kv), B(full[b]));
-        };
-        uint32_t id = page_of(0), id1 = page_of(1);
-        load(0, id, C::K, &kmap, bk_full, bk_empty);
-        for (int j = 0; j < n; j++) {
-            const uint32_t id2 = page_of(j + 2);
-            if (j + 1 < n) load(j + 1, id1, C::K, &kmap, bk_full, bk_empty);
-            load(j, id, C::V, &vmap, bv_full, bv_empty);
-            id = id1;
-            id1 = id2;
+            if (values && x.keys % 128) {
+                const int b = (t - 1) % C::STAGES, keep = (int)(x.keys % 128);
+                mbar_wait(B(bv_full[b]), ((t - 1) / C::STAGES) & 1, err, &gave_up);
+                // The clear before has been used: its stage's next copy waited for that, or else this does.
+                if (last_clear >= 0 && t - 1 < last_clear + C::STAGES)
+                    mbar_wait(B(bv_empty[last_clear % C::STAGES]), (last_clear / C::STAGES) & 1, err, &gave_up);
+                last_clear = t - 1;
+                uint8_t *vt = smem + C::V + b * C::TILE;
+                for (int i = lane; i < C::HALVES * (128 - keep) * 8; i += 32) {
+                    const int c = i / ((128 - keep) * 8), r = keep + i / 8 % (128 - keep);  // a swizzled row is 128 whole bytes
+                    *reinterpret_cast<uint4 *>(vt + c * C::HALF + r * 128 + (i % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // for the tensor cores' reads
+                __syncwarp();
+                if (lane == 0) mbar_arrive(B(bv_clear));
+            }
         }
         // Every copy has landed before the block can end.
-        for (int j = n > C::STAGES ? n - C::STAGES : 0; j < n; j++) {
-            mbar_wait(B(bk_full[j % C::STAGES]), (j / C::STAGES) & 1, err, &gave_up);
-            mbar_wait(B(bv_full[j % C::STAGES]), (j / C::STAGES) & 1, err, &gave_up);
-        }
-        mbar_wait(B(bq), 0, err, &gave_up);
-        if (clear_v) {
-            uint8_t *vt = smem + C::V + ((n - 1) % C::STAGES) * C::TILE;
-            const int keep = (int)(keys % 128);
-            for (int i = lane; i < C::HALVES * (128 - keep) * 8; i += 32) {
-                const int c = i / ((128 - keep) * 8), r = keep + i / 8 % (128 - keep);  // a swizzled row is 128 whole bytes
-                *reinterpret_cast<uint4 *>(vt + c * C::HALF + r * 128 + (i % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // for the tensor cores' reads
-            __syncwarp();
-            if (lane == 0) mbar_arrive(B(bv_clear));
-        }
+        for (int i = t > C::STAGES ? t - C::STAGES : 0; i < t; i++) mbar_wait(B(full[i % C::STAGES]), (i / C::STAGES) & 1, err, &gave_up);
+        if (warp == 0) mbar_wait(B(bq_full), (done - 1) & 1, err, &gave_up);
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc_s = bf16_idesc(128, 128);
             constexpr uint32_t idesc_o = bf16_idesc(128, HD) | (1u << 16);  // B (V) MN-major
-            auto issue_s = [&](int j, int h) {
-                const uint32_t kt = base + C::K + (j % C::STAGES) * C::TILE, qt = base + C::Q + h * C::TILE;
+            int t0 = 0, done = 0, cleared = 0, seen[2] = {0, 0};  // seen: the tiles of keys each tile of queries has had
+            for (uint32_t u = blockIdx.x; u < units; u += gridDim.x, done++) {
+                const Unit x = unit(u);
+                auto issue_s = [&](int j, int h) {
+                    const uint32_t kt = base + C::K + ((t0 + j) % C::STAGES) * C::TILE, qt = base + C::Q + h * C::TILE;
+                    const int at_s = seen[h] + j;
 #pragma unroll
-                for (int i = 0; i < HD / 16; i++)
-                    tc_mma(tmem + C::s_col(h, j), sw128_desc(qt + (i / 4) * C::HALF + (i % 4) * 32),
-                           sw128_desc(kt + (i / 4) * C::HALF + (i % 4) * 32), idesc_s, i > 0 ? 1u : 0u);
-                tc_commit(B(bs_full[h * C::SB + (C::SB - 1) * (j & 1)]));
-            };
-            auto wait_k = [&](int j) {
-                mbar_wait(B(bk_full[j % C::STAGES]), (j / C::STAGES) & 1, err, &gave_up);
-                tc_fence_after();
-            };
-            mbar_wait(B(bq), 0, err, &gave_up);
-            for (int j = 0; j < C::SB && j < n; j++) {
-                wait_k(j);
-                for (int h = 0; h < nt; h++) issue_s(j, h);
-                tc_commit(B(bk_empty[j % C::STAGES]));
-            }
-            for (int j = 0; j < n; j++) {
-                const int b = j % C::STAGES, next = j + C::SB;  // the S whose buffer S_j leaves free
-                const uint32_t v = base + C::V + b * C::TILE;
-                for (int h = 0; h < nt; h++) {
-                    // P_j in TMEM, S_j read, and O rescaled to the query's reference.
-                    mbar_wait(B(bp_full[h]), j & 1, err, &gave_up);
+                    for (int i = 0; i < HD / 16; i++)
+                        tc_mma(tmem + C::s_col(h, at_s), sw128_desc(qt + (i / 4) * C::HALF + (i % 4) * 32),
+                               sw128_desc(kt + (i / 4) * C::HALF + (i % 4) * 32), idesc_s, i > 0 ? 1u : 0u);
+                    tc_commit(B(bs_full[h * C::SB + (C::SB - 1) * (at_s & 1)]));
+                };
+                auto wait_k = [&](int j) {
+                    mbar_wait(B(bk_full[(t0 + j) % C::STAGES]), ((t0 + j) / C::STAGES) & 1, err, &gave_up);
                     tc_fence_after();
-                    if (C::SB == 1 && next < n) {
-                        if (h == 0) wait_k(next);
-                        issue_s(next, h);
-                        if (h == nt - 1) tc_commit(B(bk_empty[next % C::STAGES]));
-                    }
-                    if (h == 0) {
-                        mbar_wait(B(bv_full[b]), (j / C::STAGES) & 1, err, &gave_up);
-                        if (clear_v && j == n - 1) mbar_wait(B(bv_clear), 0, err, &gave_up);
+                };
+                mbar_wait(B(bq_full), done & 1, err, &gave_up);
+                for (int j = 0; j < C::SB && j < x.n; j++) {
+                    wait_k(j);
+                    for (int h = 0; h < x.nt; h++) issue_s(j, h);
+                    tc_commit(B(bk_empty[(t0 + j) % C::STAGES]));
+                }
+                for (int j = 0; j < x.n; j++) {
+                    const int b = (t0 + j) % C::STAGES, next = j + C::SB;  // the S whose buffer S_j leaves free
+                    const uint32_t v = base + C::V + b * C::TILE;
+                    for (int h = 0; h < x.nt; h++) {
+                        // P_j in TMEM, S_j read, and O rescaled to the query's reference (or the unit's before stored).
+                        mbar_wait(B(bp_full[h]), (seen[h] + j) & 1, err, &gave_up);
                         tc_fence_after();
-                    }
+                        if (C::SB == 1 && next < x.n) {
+                            if (h == 0) wait_k(next);
+                            issue_s(next, h);
+                            if (h == x.nt - 1) tc_commit(B(bk_empty[(t0 + next) % C::STAGES]));
+                        }
+                        if (h == 0) {
+                            mbar_wait(B(bv_full[b]), ((t0 + j) / C::STAGES) & 1, err, &gave_up);
+                            if (j == x.n - 1 && x.keys % 128) mbar_wait(B(bv_clear), cleared++ & 1, err, &gave_up);
+                            tc_fence_after();
+                        }
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        tc_mma_ts(tmem + C::o_col(h), tmem + C::p_col(h) + 8 * i, mn_desc(v + i * 2048, C::HALF), idesc_o,
-                                  (j > 0 || i > 0) ? 1u : 0u);
-                    tc_commit(B(bo_full[h]));
+                        for (int i = 0; i < 8; i++)
+                            tc_mma_ts(tmem + C::o_col(h), tmem + C::p_col(h) + 8 * i, mn_desc(v + i * 2048, C::HALF), idesc_o,
+                                      (j > 0 || i > 0) ? 1u : 0u);
+                        tc_commit(B(bo_full[h]));
+                    }
+                    tc_commit(B(bv_empty[b]));
+                    if (C::SB == 2 && next < x.n) {
+                        wait_k(next);
+                        issue_s(next, 0);
+                        tc_commit(B(bk_empty[(t0 + next) % C::STAGES]));
+                    }
                 }
-                tc_commit(B(bv_empty[b]));
-                if (C::SB == 2 && next < n) {
-                    wait_k(next);
-                    issue_s(next, 0);
-                    tc_commit(B(bk_empty[next % C::STAGES]));
-                }
+                t0 += x.n;
+                for (int h = 0; h < x.nt; h++) seen[h] += x.n;
             }
         }
-    } else if ((warp - 2) / 4 < nt) {
+    } else {
         const int h = (warp - 2) / 4, quad = warp & 3, m = quad * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         const float scale2 = 1.4426950408889634f / sqrtf((float)HD);  // log2(e) / sqrt(hd)
-        float mref = -INFINITY, l = 0.0f;
-        for (int j = 0; j < n; j++) {
-            mbar_wait(B(bs_full[h * C::SB + (C::SB - 1) * (j & 1)]), (j / C::SB) & 1, err, &gave_up);
-            tc_fence_after();
-            const int live = (int)keys - j * 128;
-            // P_j against mref into TMEM with its sum, the tile's raw maximum alongside; P_j takes
-            // P_{j-1}'s place once PV_{j-1} has read it, which the first pass waits for.
-            auto p_pass = [&](float &mx, bool first) {
-                float2 sum4[4];
+        int t = 0;  // the tiles of keys this tile of queries has had
+        for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
+            const Unit x = unit(u);
+            if (h < x.nt) {
+                float mref = -INFINITY, l = 0.0f;
+                // 32 columns of S_j on their way, and as scores, past the prefix -inf. (The passes are loops of such steps, two to
+                // a turn, not unrolled over a tile: the first tile waits for their code.)
+                uint32_t r[2][2][16];
+                auto fetch = [&](int c, uint32_t (&to)[2][16]) {
+                    tmem_ld16_nowait(lanes + C::s_col(h, t) + (uint32_t)c, to[0]);
+                    tmem_ld16_nowait(lanes + C::s_col(h, t) + (uint32_t)c + 16, to[1]);
+                };
+                auto scores = [&](int j, int c, const uint32_t (&from)[2][16], float (&sv)[32]) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) sum4[e] = make_float2(0.0f, 0.0f);
-                float mxs[2] = {-INFINITY, -INFINITY};
-                const float nm = mref != -INFINITY ? -mref : -INFINITY;  // every score -inf: P comes out 0
-                const float2 scale22 = make_float2(scale2, scale2), neg_m = make_float2(nm, nm);
+                    for (int i = 0; i < 32; i++) sv[i] = __uint_as_float(from[i / 16][i % 16]);
+                    const int live = (int)x.keys - j * 128 - c;
+                    if (live < 32) {
 #pragma unroll
-                for (int c2 = 0; c2 < 2; c2++) {
-                    uint32_t r[4][16];
-#pragma unroll
-                    for (int c = 0; c < 4; c++) tmem_ld16_nowait(lanes + C::s_col(h, j) + (uint32_t)(c2 * 64 + c * 16), r[c]);
-                    tmem_wait_ld();
-                    float sv[64];
-#pragma unroll
-                    for (int c = 0; c < 64; c++) sv[c] = __uint_as_float(r[c / 16][c % 16]);
-                    if (c2 * 64 + 64 > live) {
-#pragma unroll
-                        for (int c = 0; c < 64; c++)
-                            if (c2 * 64 + c >= live) sv[c] = -INFINITY;
+                        for (int i = 0; i < 32; i++)
+                            if (i >= live) sv[i] = -INFINITY;
                     }
-                    uint32_t pk[2][16];
+                };
+                for (int j = 0; j < x.n; j++, t++) {
+                    mbar_wait(B(bs_full[h * C::SB + (C::SB - 1) * (t & 1)]), (t / C::SB) & 1, err, &gave_up);
+                    tc_fence_after();
+                    if (j == 0) {  // no reference yet: the tile's maximum first
+                        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+                        for (int c = 0; c < 128; c += 32) {
+                            fetch(c, r[0]);
+                            tmem_wait_ld();
+                            float sv[32];
+                            scores(0, c, r[0], sv);
 #pragma unroll
-                    for (int c = 0; c < 64; c += 2) {
-                        mxs[(c / 2) % 2] = max3(mxs[(c / 2) % 2], sv[c], sv[c + 1]);
-                        const float2 x = fma2(make_float2(sv[c], sv[c + 1]), scale22, neg_m);
-                        const float p0 = hw_exp2(x.x), p1 = hw_exp2(x.y);
-                        sum4[(c % 8) / 2] = add2(sum4[(c % 8) / 2], make_float2(p0, p1));
-                        pk[c / 32][(c / 2) % 16] = fa::pack_bf16(p0, p1);
+                            for (int i = 0; i < 32; i += 2) mx[(i / 2) % 2] = max3(mx[(i / 2) % 2], sv[i], sv[i + 1]);
+                        }
+                        mref = fmaxf(mx[0], mx[1]) * scale2;
                     }
-                    if (c2 == 0 && first && j > 0) {
-                        mbar_wait(B(bo_full[h]), (j - 1) & 1, err, &gave_up);
-                        tc_fence_after();
+                    // P_j against mref into TMEM with its sum, the tile's raw maximum alongside; P_j takes P_{j-1}'s place once
+                    // PV_{j-1} has read it. Where the maximum has passed a reference by MOVE_PAST, O (with PV_{j-1} in it) is
+                    // rescaled, a query that keeps its reference times 1, and the warp's pass runs again from S_j.
+                    float a = 1.0f, sum;
+                    for (bool again = false;; again = true) {
+                        float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                        float mx[2] = {-INFINITY, -INFINITY};
+                        const float nm = mref != -INFINITY ? -mref : -INFINITY;  // every score -inf: P comes out 0
+                        const float2 scale22 = make_float2(scale2, scale2), neg_m = make_float2(nm, nm);
+                        fetch(0, r[0]);
+#pragma unroll 1
+                        for (int c2 = 0; c2 < 128; c2 += 64) {
+#pragma unroll
+                            for (int z = 0; z < 2; z++) {
+                                const int c = c2 + 32 * z;
+                                tmem_wait_ld();
+                                if (c + 32 < 128) fetch(c + 32, r[1 - z]);
+                                float sv[32];
+                                scores(j, c, r[z], sv);
+                                uint32_t pk[16];
+#pragma unroll
+                                for (int i = 0; i < 32; i += 2) {
+                                    mx[(i / 2) % 2] = max3(mx[(i / 2) % 2], sv[i], sv[i + 1]);
+                                    const float2 e = fma2(make_float2(sv[i], sv[i + 1]), scale22, neg_m);
+                                    const float p0 = hw_exp2(e.x), p1 = hw_exp2(e.y);
+                                    sums[(i / 2) % 2] = add2(sums[(i / 2) % 2], make_float2(p0, p1));
+                                    pk[i / 2] = fa::pack_bf16(p0, p1);
+                                }
+                                if (c == 0 && !again && j > 0) {
+                                    mbar_wait(B(bo_full[h]), (t - 1) & 1, err, &gave_up);
+                                    tc_fence_after();
+                                }
+                                tmem_st16(lanes + C::p_col(h) + (uint32_t)(c / 2), pk);
+                            }
+                        }
+                        sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+                        const float m_tile = fmaxf(mx[0], mx[1]) * scale2;
+                        const bool move = m_tile > mref + MOVE_PAST;
+                        if (again || !__any_sync(0xffffffffu, move)) break;
+                        a = move && mref != -INFINITY ? hw_exp2(mref - m_tile) : 1.0f;
+                        if (move) mref = m_tile;
+                        tmem_wait_st();
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16_nowait(lanes + C::o_col(h) + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+                            tmem_st16(lanes + C::o_col(h) + c, o);
+                        }
+                        tmem_wait_st();
                     }
-                    tmem_st16(lanes + C::p_col(h) + 32 * c2, pk[0]);
-                    tmem_st16(lanes + C::p_col(h) + 32 * c2 + 16, pk[1]);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    l = __fmaf_rn(l, a, sum);
+                    mbar_arrive(B(bp_full[h]));
                 }
-                mx = fmaxf(mxs[0], mxs[1]);
-                return ((sum4[0].x + sum4[0].y) + (sum4[1].x + sum4[1].y)) +
-                       ((sum4[2].x + sum4[2].y) + (sum4[3].x + sum4[3].y));
-            };
-            if (j == 0) {  // no reference yet: the tile's maximum first
-                float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c4 = 0; c4 < 2; c4++) {
-                    uint32_t r[4][16];
-#pragma unroll
-                    for (int c = 0; c < 4; c++) tmem_ld16_nowait(lanes + C::s_col(h, 0) + (uint32_t)(c4 * 64 + c * 16), r[c]);
+                mbar_wait(B(bo_full[h]), (t - 1) & 1, err, &gave_up);
+                tc_fence_after();
+                // The partials, where a query is one: O as it stands in TMEM by way of shared memory (the Q tile: every S
+                // of the unit is done once its last PV is), so that a store covers whole lines of four queries;
+                // references and sums. A row of the stage is 32 values, its 16-byte pieces turned by the row.
+                const int row = (x.tile0 + h) * tile_rows + m / group;
+                const bool real = m < tile_rows * group && row < (int)p.rows;
+                const uint64_t to = real ? ((uint64_t)row * heads + x.kv * group + m % group) * pieces + x.piece : ~0ull;
+                float4 *stage = reinterpret_cast<float4 *>(smem + C::Q + h * C::TILE + quad * 4096);
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[2][16];
+                    tmem_ld16_nowait(lanes + C::o_col(h) + c, o[0]);
+                    tmem_ld16_nowait(lanes + C::o_col(h) + c + 16, o[1]);
                     tmem_wait_ld();
-                    const int in = min(live - c4 * 64, 64);
 #pragma unroll
-                    for (int c = 0; c < 64; c += 2)
-                        mxs[(c / 2) % 4] = max3(mxs[(c / 2) % 4], c < in ? __uint_as_float(r[c / 16][c % 16]) : -INFINITY,
-                                                c + 1 < in ? __uint_as_float(r[c / 16][c % 16 + 1]) : -INFINITY);
+                    for (int e = 0; e < 8; e++)
+                        stage[lane * 8 + (e ^ (lane & 7))] =
+                            make_float4(__uint_as_float(o[e / 4][e % 4 * 4]), __uint_as_float(o[e / 4][e % 4 * 4 + 1]),
+                                        __uint_as_float(o[e / 4][e % 4 * 4 + 2]), __uint_as_float(o[e / 4][e % 4 * 4 + 3]));
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int q = 4 * i + lane / 8;
+                        const uint64_t dst = __shfl_sync(0xffffffffu, to, q);
+                        if (dst != ~0ull) *reinterpret_cast<float4 *>(out.o + dst * HD + c + 4 * (lane % 8)) = stage[q * 8 + (lane % 8 ^ (q & 7))];
+                    }
+                    __syncwarp();
                 }
-                mref = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * scale2;
+                if (real) *reinterpret_cast<float2 *>(out.ml + to * 2) = make_float2(mref, l);
+                tc_fence_before();
+                if (blank) {  // as Q expects it, once every warp of the tile is done with its part of the stage
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + h) : "memory");
+                    blank_q(h, m, 128);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next Q's copies
             }
-            float a = 1.0f, mx;
-            float sum = p_pass(mx, true);
-            const float m_tile = mx * scale2;
-            const bool move = m_tile > mref + MOVE_PAST;
-            if (__any_sync(0xffffffffu, move)) {
-                // A query of the warp moves: O (with PV_{j-1} in it) rescaled, a query that keeps its
-                // reference times 1, then the warp's P_j again from S_j, still in TMEM.
-                a = move && mref != -INFINITY ? hw_exp2(mref - m_tile) : 1.0f;
-                if (move) mref = m_tile;
-                tmem_wait_st();
-#pragma unroll
-                for (int c = 0; c < HD / 16; c++) {
-                    uint32_t o[16];
-                    tmem_ld16_nowait(lanes + C::o_col(h) + c * 16, o);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-                    tmem_st16(lanes + C::o_col(h) + c * 16, o);
-                }
-                tmem_wait_st();
-                sum = p_pass(mx, false);
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            l = __fmaf_rn(l, a, sum);
-            mbar_arrive(B(bp_full[h]));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(B(bq_empty));
         }
-        mbar_wait(B(bo_full[h]), (n - 1) & 1, err, &gave_up);
-        tc_fence_after();
-        // The partial of query m, where it is one: O as it stands in TMEM, and its reference and sum.
-        const int row = (tile0 + h) * tile_rows + m / group;
-        const bool real = m < tile_rows * group && row < (int)p.rows;
-        const size_t to = (((size_t)(real ? row : 0) * heads + kv * group + m % group) * pieces + blockIdx.x);
-#pragma unroll
-        for (int c = 0; c < HD / 16; c++) {
-            uint32_t o[16];
-            tmem_ld16_nowait(lanes + C::o_col(h) + c * 16, o);
-            tmem_wait_ld();
-            if (real) {
-                store8(out.o + to * HD + c * 16, o);
-                store8(out.o + to * HD + c * 16 + 8, o + 8);
-            }
-        }
-        if (real) *reinterpret_cast<float2 *>(out.ml + to * 2) = make_float2(mref, l);
     }
     tc_fence_before();
     __syncthreads();
@@ -670,51 +835,72 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// Joins a row's partials, a warp to a head, in piece order. References are in base 2 for bf16, natural for f32.
-// A lane takes four dimensions of every LANES-th piece, so that a warp has several pieces' loads in flight; the
-// lanes' sums are added by a butterfly.
+// Joins the partials of a row's head, a block to it: 16 bytes of a piece's o to a lane, the pieces over the
+// block's groups of HD / 4 lanes, all loads of a row of up to JOIN_DEEP pieces a group in flight at once; the
+// groups' sums are then added in order. References are in base 2 for bf16, natural for f32.
+constexpr int JOIN_THREADS = 128, JOIN_DEEP = 8;
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(JOIN_THREADS)
     join_kernel(tg_params p, const uint32_t *__restrict__ at, Partials in, uint32_t np, uint32_t pieces, T *__restrict__ out) {
-    constexpr int LANES = 32 / (HD / 4);  // pieces at once
+    constexpr int LANES = HD / 4, GROUPS = JOIN_THREADS / LANES;
+    __shared__ __align__(16) float4 acc_s[GROUPS][LANES];
+    __shared__ float m_s[GROUPS], l_s[GROUPS];
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31, d = 4 * (lane % (HD / 4)), of = lane / (HD / 4);
-    const uint64_t item = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (item >= (uint64_t)p.rows * p.heads) return;
+    const uint64_t item = blockIdx.x;
+    const int group = threadIdx.x / LANES, d = threadIdx.x % LANES;
     uint32_t length, seq;
     if (!paged_row(p, at, (int)(item / p.heads), length, seq, nullptr)) return;
-    const uint32_t n = np + (length + own_piece(HD) - 1) / own_piece(HD);
+    const uint32_t n = np + (length + OWN_PIECE - 1) / OWN_PIECE;
     const float2 *ml = reinterpret_cast<const float2 *>(in.ml) + item * pieces;
-    const float *o = in.o + item * pieces * HD + d;
+    const float4 *o = reinterpret_cast<const float4 *>(in.o + item * pieces * HD) + d;
+    auto power = [](float x) { return sizeof(T) == 2 ? exp2f(x) : expf(x); };
     float m = -INFINITY, l = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    auto power = [](float x) { return sizeof(T) == 2 ? exp2f(x) : expf(x); };
-    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
-        // 32 pieces at once: a lane holds one's reference and sum.
-        const float2 part = i0 + lane < n ? ml[i0 + lane] : make_float2(-INFINITY, 0.0f);
-        const float next = fmaxf(m, warp_max(part.x)), keep = m == -INFINITY ? 0.0f : power(m - next);
-        const float e = part.x == -INFINITY ? 0.0f : power(part.x - next);
+    for (uint32_t i0 = group; i0 < n; i0 += GROUPS * JOIN_DEEP) {
+        float2 part[JOIN_DEEP];
+        float4 x[JOIN_DEEP];
+#pragma unroll
+        for (int i = 0; i < JOIN_DEEP; i++) {
+            const uint32_t piece = i0 + i * GROUPS;
+            part[i] = piece < n ? ml[piece] : make_float2(-INFINITY, 0.0f);
+            x[i] = piece < n ? o[(size_t)piece * LANES] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        float next = m;
+#pragma unroll
+        for (int i = 0; i < JOIN_DEEP; i++) next = fmaxf(next, part[i].x);
+        const float keep = m == -INFINITY ? 0.0f : power(m - next);
         m = next;
-        l = __fmaf_rn(l, keep, warp_sum(part.y * e));
+        l *= keep;
         acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
-        const uint32_t count = min(n - i0, 32u);
-#pragma unroll 4
-        for (uint32_t i = 0; i < count; i += LANES) {
-            const float w = __shfl_sync(0xffffffffu, e, (i + of) & 31);
-            if (i + of >= count) continue;
-            const float4 x = *reinterpret_cast<const float4 *>(o + (size_t)(i0 + i + of) * HD);
-            acc = make_float4(__fmaf_rn(x.x, w, acc.x), __fmaf_rn(x.y, w, acc.y), __fmaf_rn(x.z, w, acc.z), __fmaf_rn(x.w, w, acc.w));
+#pragma unroll
+        for (int i = 0; i < JOIN_DEEP; i++) {
+            const float e = part[i].x == -INFINITY ? 0.0f : power(part[i].x - m);
+            l = __fmaf_rn(part[i].y, e, l);
+            acc = make_float4(__fmaf_rn(x[i].x, e, acc.x), __fmaf_rn(x[i].y, e, acc.y), __fmaf_rn(x[i].z, e, acc.z), __fmaf_rn(x[i].w, e, acc.w));
         }
     }
-    if (LANES > 1) {
-        acc.x += __shfl_xor_sync(0xffffffffu, acc.x, 16);
-        acc.y += __shfl_xor_sync(0xffffffffu, acc.y, 16);
-        acc.z += __shfl_xor_sync(0xffffffffu, acc.z, 16);
-        acc.w += __shfl_xor_sync(0xffffffffu, acc.w, 16);
+    // The groups' references joined, then their sums.
+    if (d == 0) m_s[group] = m;
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < GROUPS; i++) top = fmaxf(top, m_s[i]);
+    const float e = m == -INFINITY ? 0.0f : power(m - top);
+    if (d == 0) l_s[group] = l * e;
+    acc_s[group][d] = make_float4(acc.x * e, acc.y * e, acc.z * e, acc.w * e);
+    __syncthreads();
+    if (group) return;
+    l = 0.0f;
+    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < GROUPS; i++) {
+        const float4 x = acc_s[i][d];
+        l += l_s[i];
+        acc = make_float4(acc.x + x.x, acc.y + x.y, acc.z + x.z, acc.w + x.w);
     }
-    if (of) return;
-    T *dst = out + item * HD + d;
+    T *dst = out + item * HD + 4 * d;
     const float4 r = make_float4(__fdiv_rn(acc.x, l), __fdiv_rn(acc.y, l), __fdiv_rn(acc.z, l), __fdiv_rn(acc.w, l));
     if constexpr (sizeof(T) == 2)
         *reinterpret_cast<uint2 *>(dst) = make_uint2(fa::pack_bf16(r.x, r.y), fa::pack_bf16(r.z, r.w));
@@ -736,7 +922,7 @@ bool map_heads(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t outer,
 
 template <typename T, int HD>
 cudaError_t attend(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at, const uint32_t *table,
-                   const uint32_t *shared, void *work, void *out, uint32_t *err, cudaStream_t s) {
+                   const uint32_t *shared, void *work, void *out, uint32_t *err, int sm_count, cudaStream_t s) {
     const uint64_t pieces = all_pieces(p), items = (uint64_t)p.rows * p.heads;
     if (pieces > 0x7fffffffu || p.kv_heads > 65535) return cudaErrorNotSupported;
     float *o = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(work) + 255) & ~uintptr_t(255));
@@ -755,38 +941,42 @@ cudaError_t attend(const tg_params &p, const void *q, const void *k, const void 
                 return cudaErrorInvalidValue;
             e = with_smem(prefix_kernel<HD>, C::SMEM);
             if (e != cudaSuccess) return e;
-            const uint32_t tiles = (p.rows + tile_rows - 1) / tile_rows;
-            e = launch_pdl(prefix_kernel<HD>, dim3(np, (tiles + C::NT - 1) / C::NT, p.kv_heads), dim3(C::THREADS), C::SMEM, s, qm, km,
+            const uint32_t tiles = (p.rows + tile_rows - 1) / tile_rows, units = np * ((tiles + C::NT - 1) / C::NT) * p.kv_heads;
+            e = launch_pdl(prefix_kernel<HD>, dim3(std::min(units, (uint32_t)sm_count)), dim3(C::THREADS), C::SMEM, s, qm, km,
                            vm, p, at, shared, part, (uint32_t)pieces, box, err);
             if (e != cudaSuccess) return e;
         }
-        e = with_smem(own_kernel<HD>, own_smem(HD));
+        CUtensorMap km, vm;
+        if (!map_heads(&km, k, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, 16, 1) ||
+            !map_heads(&vm, v, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, 16, 1))
+            return cudaErrorInvalidValue;
+        e = with_smem(own_kernel<HD>, OWN_SMEM);
         if (e != cudaSuccess) return e;
-        e = launch_pdl(own_kernel<HD>, dim3((unsigned)(pieces - np), p.kv_heads, p.rows), dim3(OWN_WARPS * 32), own_smem(HD), s, p,
-                       (const T *)q, (const T *)k, (const T *)v, at, table, part, np, (uint32_t)pieces, err);
+        const uint64_t most = (uint64_t)p.rows * p.kv_heads * (pieces - np);
+        e = launch_pdl(own_kernel<HD>, dim3((unsigned)std::min<uint64_t>(most, (uint64_t)sm_count * OWN_BLOCKS)), dim3(32), OWN_SMEM, s, km,
+                       vm, p, (const T *)q, at, table, part, np, (uint32_t)pieces, err);
     } else {
         e = launch_pdl(pieces_kernel<T, HD>, dim3((unsigned)pieces, p.kv_heads, p.rows), dim3(CHUNK), 0, s, p, (const T *)q, (const T *)k,
                        (const T *)v, at, table, shared, part, np, (uint32_t)pieces, err);
     }
     if (e != cudaSuccess) return e;
-    return launch_pdl(join_kernel<T, HD>, dim3((unsigned)((items + 3) / 4)), dim3(128), 0, s, p, at, part, np, (uint32_t)pieces, (T *)out);
+    return launch_pdl(join_kernel<T, HD>, dim3((unsigned)items), dim3(JOIN_THREADS), 0, s, p, at, part, np, (uint32_t)pieces, (T *)out);
 }
 
 }  // namespace
 
 uint64_t attention_pages_work(const tg_params &p) {
-    if (p.head_dim == 0 || p.head_dim > 16384) return 0;
     return (uint64_t)p.rows * p.heads * all_pieces(p) * (p.head_dim + 2) * sizeof(float) + 256;
 }
 
 cudaError_t launch_attention_pages(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at,
                                    const uint32_t *table, const uint32_t *shared, void *work, void *out, uint32_t *err,
-                                   cudaStream_t s) {
+                                   int sm_count, cudaStream_t s) {
     if (p.dtype == TG_BF16)
-        return p.head_dim == 64 ? attend<bf16, 64>(p, q, k, v, at, table, shared, work, out, err, s)
-                                : attend<bf16, 128>(p, q, k, v, at, table, shared, work, out, err, s);
-    return p.head_dim == 64 ? attend<float, 64>(p, q, k, v, at, table, shared, work, out, err, s)
-                            : attend<float, 128>(p, q, k, v, at, table, shared, work, out, err, s);
+        return p.head_dim == 64 ? attend<bf16, 64>(p, q, k, v, at, table, shared, work, out, err, sm_count, s)
+                                : attend<bf16, 128>(p, q, k, v, at, table, shared, work, out, err, sm_count, s);
+    return p.head_dim == 64 ? attend<float, 64>(p, q, k, v, at, table, shared, work, out, err, sm_count, s)
+                            : attend<float, 128>(p, q, k, v, at, table, shared, work, out, err, sm_count, s);
 }
 
 }  // namespace tg

@@ -519,7 +519,7 @@ int enqueue_launch(const Launch &l, uint32_t *err, cudaStream_t s, int sm_count)
         case TG_KERNEL_DIT_EULER: e = launch_dit_euler(p, b[0], b[1], b[2], F(3), F(4), s); break;
         case TG_KERNEL_PAGE_PLAN: e = launch_page_plan(p, U(0), U(1), U(2), U(3), U(4), U(5), U(6), U(7), U(8), err, s); break;
         case TG_KERNEL_ROPE_PAGES: e = launch_rope_pages(p, U(0), U(1), b[2], F(3), F(4), b[5], b[6], b[7], err, s); break;
-        case TG_KERNEL_ATTENTION_PAGES: e = launch_attention_pages(p, b[0], b[1], b[2], U(3), U(4), U(5), b[6], b[7], err, s); break;
+        case TG_KERNEL_ATTENTION_PAGES: e = launch_attention_pages(p, b[0], b[1], b[2], U(3), U(4), U(5), b[6], b[7], err, sm_count, s); break;
         case TG_KERNEL_LOGITS_PICK: e = launch_logits_pick(p, b[0], U(1), U(2), F(3), U(4), F(5), U(6), b[7], U(8), err, s); break;
         default: return fail(TG_EINVAL, "no kernel %u", l.kernel);
     }

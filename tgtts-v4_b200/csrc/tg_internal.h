@@ -245,7 +245,7 @@ cudaError_t launch_rope_pages(const tg_params &p, const uint32_t *at, const uint
                               cudaStream_t s);
 cudaError_t launch_attention_pages(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at,
                                    const uint32_t *table, const uint32_t *shared, void *work, void *out, uint32_t *err,
-                                   cudaStream_t s);
+                                   int sm_count, cudaStream_t s);
 uint64_t attention_pages_work(const tg_params &p);
 cudaError_t launch_logits_pick(const tg_params &p, const void *logits, const uint32_t *seen, const uint32_t *spans,
                                const float *penalties, const uint32_t *bias_ids, const float *bias,
