@@ -38,9 +38,6 @@ __host__ __device__ inline uint64_t all_pieces(const tg_params &p) {
 struct Partials {
     float *o, *ml;
 };
-// Behind them own_kernel's counters, one to a list of OWN_ROWS rows.
-constexpr uint32_t OWN_ROWS = 192;
-__host__ __device__ inline uint32_t own_lists(uint32_t rows) { return (rows + OWN_ROWS - 1) / OWN_ROWS; }
 
 // A row's own length and request; false for a row that computes nothing.
 TG_DEVICE bool paged_row(const tg_params &p, const uint32_t *at, int row, uint32_t &length, uint32_t &seq, uint32_t *err) {
@@ -179,6 +176,10 @@ TG_DEVICE float hw_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Brings a copy's descriptor near before its first use.
+TG_DEVICE void prefetch_map(const CUtensorMap *map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 // A tile [keys][64 to a chunk] read with its 64-dimension chunks (`chunk` bytes apart) as M or N and its keys as K: atoms of
 // 8 keys x 128 bytes, 1024 bytes apart.
 TG_DEVICE uint64_t mn_desc(uint32_t addr, uint32_t chunk) {
@@ -187,314 +188,213 @@ TG_DEVICE uint64_t mn_desc(uint32_t addr, uint32_t chunk) {
 }
 
 // ---- own pieces, bf16 ---------------------------------------------------------------------------------
-// A unit is a piece of up to 128 of a row's own positions, for one KV head of 128 dimensions or two of 64 (so that a
-// tile of keys or values is 128 positions x 2 chunks of 64 either way). The positions are the rows of the products, the
-// group's query heads (at most 8) their columns:
-//   S^T = K q^T      (M = 128 positions, N = 16, K = HD; for HD = 64 once a KV head)
-//   O^T = V^T e^T    (M = 128: HD dimensions, or the 64 of two KV heads; K = positions; N: the heads' e as bf16 hi, then
-//                    as lo = e - hi, so that e keeps 16 bits)
-// so keys and values go from TMA's tiles to the tensor cores and a thread handles one position's scores. Six warps:
-//   warps 0-3  a thread to a position: scores, the heads' maxima over the block, e and their sums, e into shared memory;
-//              then O^T of the unit, a thread to a dimension, stored in whole lines;
-//   warp 4     the MMAs (and zeros in the last 16 positions' values past the row's length: 0 x NaN is NaN);
-//   warp 5     takes the next unit, TMA: keys and queries once S^T has read the last, values once O^T has.
-// Bound by the caches' bytes: OWN_BLOCKS blocks an SM, each with up to 64 KiB on their way. (A warp to a piece on
-// mma.sync, at 376 instructions a warp and 8 KiB, reached 3.9 TB/s.) Units come off a list of the live pieces that each
-// block makes from the rows' lengths by a scan; behind prefix_kernel, whose blocks take all of an SM's TMEM, in the order
-// blocks ask for them (a counter that kernel zeroes), else each gridDim-th.
-constexpr int OWN_THREADS = 192;
+// A warp to a piece of a row's own positions for one KV head, in chunks of own_chunk positions: the group's
+// query heads, at most 8, are the columns of mma.sync.m16n8k16 (S^T = K q^T, O^T = V^T e^T with e split
+// into bf16 hi + lo, against a reference that moves as prefix_kernel's), keys and values gathered from their
+// pages by cp.async, OWN_STAGES - 1 chunks ahead of the products.
+constexpr int OWN_WARPS = 2, OWN_STAGES = 2;
+constexpr uint32_t OWN_ROWS = 512;  // rows whose pieces are listed at once
+constexpr int own_chunk(int hd) { return 2048 / hd; }
+constexpr int OWN_STAGE = 2 * 2048;  // bf16 of a chunk's keys and values
+constexpr int OWN_SMEM = OWN_WARPS * OWN_STAGES * OWN_STAGE * 2 + (int)OWN_ROWS * 4;
+constexpr int OWN_BLOCKS = 6;  // an SM's, by their shared memory
+// 16 bytes c of row r of a chunk, as an element: the rows' pieces turned so that eight rows' same piece lie in all banks.
 template <int HD>
-struct Own {
-    static constexpr int KVS = 128 / HD, NH = 8 * KVS;         // KV heads of a unit, their query heads (some blank)
-    static constexpr int NP = 2 * NH;                          // columns of e^T: hi and lo
-    static constexpr uint32_t HALF = 128 * 128, TILE = 2 * HALF;  // 128 positions of 64 dimensions; of the unit's two
-    static constexpr uint32_t K = 0, V = TILE, P = 2 * TILE, P_HALF = NP * 128, Q = P + 2 * P_HALF, Q_PART = 1024;
-    // (A Q part's 16 rows reach into the next part, the last one's into the list: columns that nobody reads.)
-    static constexpr uint32_t LIST = Q + 2 * Q_PART, SMEM = LIST + OWN_ROWS * 12 + 1024;
-    static constexpr uint32_t S_COLS = 16 * KVS, O_COL = S_COLS, COLS = 2 * S_COLS;  // TMEM: S^T, O^T
-    static constexpr int BLOCKS = HD == 64 ? 2 : 3;  // an SM's, by their shared memory
-};
-static_assert(Own<64>::COLS == 64 && Own<128>::COLS == 32 && Own<128>::NP == 16 && Own<64>::NP == 32, "TMEM columns of a unit");
+TG_DEVICE int own_at(int r, int c) { return r * HD + ((c ^ (r & 7)) << 3); }
 
-TG_DEVICE float warp_max_f32(float v) {
-    float r;
-    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
+// An 8 x 8 block of 16-bit values over a warp (lane 4 r + c: columns 2 c and 2 c + 1 of row r), transposed.
+TG_DEVICE uint32_t turn8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 template <int HD>
-__global__ void __launch_bounds__(OWN_THREADS)
-    own_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-               const __grid_constant__ CUtensorMap vmap, tg_params p, const uint32_t *__restrict__ at,
-               const uint32_t *__restrict__ table, Partials out, uint32_t np, uint32_t pieces, uint32_t box, uint32_t *counter,
-               uint32_t *err) {
-    using C = Own<HD>;
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t base = smem_u32(smem);
-    constexpr int SLOTS = 4;  // units known at once
-    __shared__ __align__(8) uint64_t bk_full, bv_full, bs_full, bp_full, bo_full, bo_read, taken[SLOTS];
-    __shared__ uint32_t tmem_slot, unit_s[SLOTS], total_s;
-    __shared__ int gave_up;
-    __shared__ float top_s[2][4][C::NH], sum_s[2][4][C::NH];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
-    const int heads = p.heads, kvh = p.kv_heads, group = heads / kvh, kv_units = (kvh + C::KVS - 1) / C::KVS;
-    uint32_t *first_piece = reinterpret_cast<uint32_t *>(smem + C::LIST), *lengths = first_piece + OWN_ROWS, *requests = lengths + OWN_ROWS;
-    auto B = [](uint64_t &b) { return smem_u32(&b); };
-    if (tid == 0) {
-        gave_up = 0;
-        mbar_init(B(bk_full), 1);
-        mbar_init(B(bv_full), 1);
-        mbar_init(B(bs_full), 1);
-        mbar_init(B(bp_full), 128);
-        mbar_init(B(bo_full), 1);
-        mbar_init(B(bo_read), 128);
-        for (int i = 0; i < SLOTS; i++) mbar_init(B(taken[i]), 1);
-        mbar_fence_init();
-    }
-    if (warp == 4) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::COLS)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+__global__ void __launch_bounds__(OWN_WARPS * 32)
+    own_kernel(tg_params p, const bf16 *__restrict__ q, const bf16 *__restrict__ k, const bf16 *__restrict__ v,
+               const uint32_t *__restrict__ at, const uint32_t *__restrict__ table, Partials out, uint32_t np,
+               uint32_t pieces, uint32_t *err) {
+    using namespace fa;
+    extern __shared__ __align__(128) unsigned char own_mem[];
+    __shared__ uint32_t total_s;
+    constexpr int CH = own_chunk(HD), VECS = HD / 8, G16 = CH / 16, ROWS = 32 / VECS;
     // Behind prefix_kernel this one starts under it: that kernel lets it go once what comes before both has
     // ended (its own wait), and the two share nothing. A block still waits before it ends, for the join.
     if (np == 0) pdl_wait();
     pdl_launch_dependents();
-
-    uint32_t n = 0;  // units of this block so far: every barrier's phases but the claims'
-    uint32_t claims = 0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3, mi = lane >> 3, rr = lane & 7;
+    const int heads = p.heads, kvh = p.kv_heads, group = heads / kvh;
+    bf16 *stages = reinterpret_cast<bf16 *>(own_mem) + warp * OWN_STAGES * OWN_STAGE;
+    uint32_t *first_piece = reinterpret_cast<uint32_t *>(own_mem + OWN_WARPS * OWN_STAGES * OWN_STAGE * 2);
+    const float scale2 = 1.4426950408889634f / sqrtf((float)HD);
     for (uint32_t row0 = 0; row0 < p.rows; row0 += OWN_ROWS) {
+        // The pieces of rows row0 .. before each of them.
         const uint32_t rows = min(OWN_ROWS, p.rows - row0);
-        __syncthreads();  // the rows before are done with the list
+        __syncthreads();  // the rows before are done with their list
         if (warp == 0) {
-            // The list: the pieces before each row, its own length and its request.
             uint32_t total = 0;
             for (uint32_t r0 = 0; r0 < rows; r0 += 32) {
-                const uint32_t r = r0 + lane;
-                uint32_t length = 0, seq = 0;
-                if (r >= rows || !paged_row(p, at, row0 + r, length, seq, blockIdx.x == 0 ? err : nullptr)) length = 0;
-                const uint32_t count = (length + OWN_PIECE - 1) / OWN_PIECE;
-                uint32_t upto = count;
+                uint32_t length, seq, n = 0;
+                if (r0 + lane < rows && paged_row(p, at, row0 + r0 + lane, length, seq, blockIdx.x == 0 ? err : nullptr))
+                    n = (length + OWN_PIECE - 1) / OWN_PIECE;
+                uint32_t upto = n;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
                     if (lane >= o) upto += u;
                 }
-                if (r < rows) {
-                    first_piece[r] = total + upto - count;
-                    lengths[r] = length;
-                    requests[r] = seq;
-                }
+                if (r0 + lane < rows) first_piece[r0 + lane] = total + upto - n;
                 total += __shfl_sync(0xffffffffu, upto, 31);
             }
             if (lane == 0) total_s = total;
         }
-        tc_fence_before();
         __syncthreads();
-        tc_fence_after();
-        const uint32_t tmem = tmem_slot, units = total_s * kv_units;
-        struct Unit {
-            uint32_t row, in_list, number;
-            int kv, live;
-        };
-        auto find = [&](uint32_t u) {
-            Unit x;
-            const uint32_t piece = u / kv_units;
-            x.kv = (int)(u % kv_units) * C::KVS;
-            uint32_t lo = 0, hi = rows;  // the row with first_piece at most `piece`, its next above
+        const uint64_t tasks = (uint64_t)total_s * kvh;
+        for (uint64_t task = (uint64_t)blockIdx.x * OWN_WARPS + warp; task < tasks; task += (uint64_t)gridDim.x * OWN_WARPS) {
+            const uint32_t u = (uint32_t)(task / kvh);
+            const int kv = (int)(task % kvh);
+            uint32_t lo = 0, hi = rows;  // the row with first_piece at most u, its next above
             while (hi - lo > 1) {
                 const uint32_t mid = (lo + hi) / 2;
-                if (first_piece[mid] <= piece) lo = mid;
+                if (first_piece[mid] <= u) lo = mid;
                 else hi = mid;
             }
-            x.in_list = lo;
-            x.row = row0 + lo;
-            x.number = piece - first_piece[lo];
-            x.live = (int)min(lengths[lo] - x.number * OWN_PIECE, OWN_PIECE);
-            return x;
-        };
-        // The block's next unit, as warp 5 wrote it (none left: units or more).
-        auto next_unit = [&](uint32_t i) {
-            mbar_wait(B(taken[i % SLOTS]), (i / SLOTS) & 1, err, &gave_up);
-            return *(volatile uint32_t *)&unit_s[i % SLOTS];
-        };
-        if (warp == 5) {
-            // A lane to a copy: one of the tile's two chunks of 64 dimensions, one box of positions.
-            const int boxes = 128 / (int)box, seg = lane % boxes, half = lane / boxes;
-            uint32_t mine = 0;
-            for (;; claims++) {
-                uint32_t u;
-                if (np == 0) u = blockIdx.x + mine++ * gridDim.x;
-                else {
-                    if (lane == 0) u = atomicAdd(counter + row0 / OWN_ROWS, 1u);
-                    u = __shfl_sync(0xffffffffu, u, 0);
-                }
-                if (gave_up) u = 0xffffffffu;
-                if (lane == 0) {
-                    *(volatile uint32_t *)&unit_s[claims % SLOTS] = u;
-                    mbar_arrive(B(taken[claims % SLOTS]));
-                }
-                if (u >= units) break;
-                const Unit x = find(u);
-                const int live_boxes = (x.live + (int)box - 1) / (int)box, parts = min(C::KVS, kvh - x.kv);
-                const int chunks = HD == 64 ? parts : 2;
-                const bool copies = half < chunks && seg < live_boxes;
-                const uint32_t pos = x.number * OWN_PIECE + min(seg, live_boxes - 1) * box;
-                uint32_t id = copies ? __ldg(table + (size_t)requests[x.in_list] * p.stride + pos / p.capacity) : 0u;
+            const uint32_t row = row0 + lo, piece = u - first_piece[lo], begin = piece * OWN_PIECE;
+            const int live = (int)min(at[row] - p.first + 1 - begin, OWN_PIECE), chunks = (live + CH - 1) / CH;
+            // Where positions begin + 16 i .. lie in the caches (16 share a page): lane i < 8.
+            uint64_t from;
+            {
+                const uint32_t pos = begin + min(16 * (lane & 7), (live - 1) & ~15);
+                uint32_t id = __ldg(table + (size_t)at[p.rows + row] * p.stride + pos / p.capacity);
                 if (id >= p.slots) {
                     atomicExch(err, ERR_BAD_INDEX);
                     id = 0;
                 }
-                const int cx = HD == 64 ? 0 : 64 * half, cy = (int)(pos % p.capacity), cz = (int)(id * kvh) + x.kv + (HD == 64 ? half : 0);
-                if (n) mbar_wait(B(bs_full), (n - 1) & 1, err, &gave_up);  // S^T has read the keys and queries before
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(B(bk_full), chunks * (live_boxes * box * 128 + group * 128));
-                    for (int c = 0; c < chunks; c++)
-                        tma_load_3d(base + C::Q + c * C::Q_PART, &qmap, HD == 64 ? 0 : 64 * c, (x.kv + (HD == 64 ? c : 0)) * group, (int)x.row,
-                                    B(bk_full));
-                }
-                __syncwarp();
-                if (copies) tma_load_3d(base + C::K + half * C::HALF + seg * box * 128, &kmap, cx, cy, cz, B(bk_full));
-                if (n) mbar_wait(B(bo_full), (n - 1) & 1, err, &gave_up);  // O^T has read the values before
-                if (lane == 0) mbar_arrive_expect_tx(B(bv_full), chunks * live_boxes * box * 128);
-                __syncwarp();
-                if (copies) tma_load_3d(base + C::V + half * C::HALF + seg * box * 128, &vmap, cx, cy, cz, B(bv_full));
-                n++;
+                from = (((uint64_t)id * kvh + kv) * p.capacity + pos % p.capacity) * HD;
             }
-            claims++;
-        } else if (warp == 4) {
-            constexpr uint32_t idesc_s = bf16_idesc(128, 16);
-            constexpr uint32_t idesc_o = bf16_idesc(128, C::NP) | (1u << 15);  // A (V^T) MN-major
-            for (;; claims++, n++) {
-                const uint32_t u = next_unit(claims);
-                if (u >= units) break;
-                const Unit x = find(u);
-                mbar_wait(B(bk_full), n & 1, err, &gave_up);
-                tc_fence_after();
-                if (lane == 0) {
+            const int in_row = lane % VECS, in_group = lane / VECS;
+            auto gather = [&](int c) {
+                bf16 *ks = stages + (c % OWN_STAGES) * OWN_STAGE, *vs = ks + CH * HD;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {  // HD = 128: 8 steps of 16 dimensions; 64: 4 of each KV head
-                        const uint32_t chunk = i / 4, to = HD == 64 ? tmem + 16 * chunk : tmem;
-                        tc_mma(to, sw128_desc(base + C::K + chunk * C::HALF + (i % 4) * 32), sw128_desc(base + C::Q + chunk * C::Q_PART + (i % 4) * 32),
-                               idesc_s, (HD == 64 ? i % 4 : i) > 0 ? 1u : 0u);
+                for (int i = 0; i < G16; i++) {
+                    const uint64_t src = __shfl_sync(0xffffffffu, from, c * G16 + i) + in_group * HD + in_row * 8;
+#pragma unroll
+                    for (int j = 0; j < 16 / ROWS; j++) {
+                        const int r = 16 * i + ROWS * j + in_group, d = own_at<HD>(r, in_row);
+                        const bool ok = c * CH + r < live;
+                        const uint64_t at_src = ok ? src + ROWS * j * HD : src - in_group * HD;  // a page's first position is there
+                        cp_async16(ks + d, k + at_src, ok);
+                        cp_async16(vs + d, v + at_src, ok);
                     }
-                    tc_commit(B(bs_full));
                 }
-                __syncwarp();
-                mbar_wait(B(bv_full), n & 1, err, &gave_up);
-                const int steps = (x.live + 15) / 16;
-                if (x.live % 16) {
-                    const int dead = 16 * steps - x.live;
-                    for (int i = lane; i < 2 * dead * 8; i += 32)  // a swizzled row is 128 whole bytes
-                        *reinterpret_cast<uint4 *>(smem + C::V + i / (dead * 8) * C::HALF + (x.live + i / 8 % dead) * 128 + i % 8 * 16) =
-                            make_uint4(0u, 0u, 0u, 0u);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // for the tensor cores' reads
-                    __syncwarp();
-                }
-                mbar_wait(B(bp_full), n & 1, err, &gave_up);              // e in shared memory (and S^T read)
-                if (n) mbar_wait(B(bo_read), (n - 1) & 1, err, &gave_up);  // the unit before has its O^T out of TMEM
-                tc_fence_after();
-                if (lane == 0) {
-                    for (int i = 0; i < steps; i++)
-                        tc_mma(tmem + C::O_COL, mn_desc(base + C::V + i * 2048, C::HALF),
-                               sw128_desc(base + C::P + i / 4 * C::P_HALF + (i % 4) * 32), idesc_o, i > 0 ? 1u : 0u);
-                    tc_commit(B(bo_full));
-                }
-                __syncwarp();
+            };
+#pragma unroll
+            for (int c = 0; c < OWN_STAGES - 1; c++) {
+                if (c < chunks) gather(c);
+                cp_async_commit();
             }
-            claims++;
-        } else {
-            const float scale2 = 1.4426950408889634f / sqrtf((float)HD);
-            const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-            for (;; claims++, n++) {
-                const uint32_t u = next_unit(claims);
-                if (u >= units) break;
-                const Unit x = find(u);
-                mbar_wait(B(bs_full), n & 1, err, &gave_up);
-                tc_fence_after();
-                uint32_t r[C::KVS][16];
+            // q of the group's heads as columns g < group of the products (those past it zero).
+            uint32_t qf[HD / 16][2];
+            const bf16 *qg = q + ((size_t)row * heads + kv * group + g) * HD + 2 * t4;
 #pragma unroll
-                for (int i = 0; i < C::KVS; i++) tmem_ld16_nowait(lanes + 16 * i, r[i]);
-                tmem_wait_ld();
-                tc_fence_before();
-                float e[C::NH];
-                float(&top)[4][C::NH] = top_s[n & 1], (&sums)[4][C::NH] = sum_s[n & 1];
+            for (int s = 0; s < HD / 16; s++) {
+                qf[s][0] = g < group ? __ldg(reinterpret_cast<const uint32_t *>(qg + 16 * s)) : 0u;
+                qf[s][1] = g < group ? __ldg(reinterpret_cast<const uint32_t *>(qg + 16 * s + 8)) : 0u;
+            }
+            // A lane's heads 2 t4 and 2 t4 + 1: references, sums, and dimensions g and g + 8 of each 16 of O^T.
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[HD / 16][4];
 #pragma unroll
-                for (int h = 0; h < C::NH; h++) {
-                    e[h] = tid < x.live ? __uint_as_float(r[h / 8][h % 8]) : -INFINITY;
-                    const float m = warp_max_f32(e[h]);
-                    if (lane == 0) top[warp][h] = m;
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                // e^T into its tile: row h of hi, row NH + h of lo, 128 bytes to 64 positions, swizzled.
-                uint8_t *tile = smem + C::P + tid / 64 * C::P_HALF + tid % 8 * 2;
-                float part[C::NH];
+            for (int j = 0; j < HD / 16; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+            for (int c = 0; c < chunks; c++) {
+                cp_async_wait<OWN_STAGES - 2>();
+                __syncwarp();  // the chunk is in, and every lane is done with the one before
+                if (c + OWN_STAGES - 1 < chunks) gather(c + OWN_STAGES - 1);
+                cp_async_commit();
+                const bf16 *ks = stages + (c % OWN_STAGES) * OWN_STAGE, *vs = ks + CH * HD;
+                float sc[G16][4];  // positions g and g + 8 of each 16, the lane's two heads
+                const int left = live - c * CH - g;
 #pragma unroll
-                for (int h = 0; h < C::NH; h++) {
-                    const float m = fmaxf(fmaxf(top[0][h], top[1][h]), fmaxf(top[2][h], top[3][h])) * scale2;
-                    const float v = e[h] == -INFINITY ? 0.0f : hw_exp2(__fmaf_rn(e[h], scale2, -m));
-                    part[h] = v;
-                    const bf16 hi = __float2bfloat16_rn(v), lo = __float2bfloat16_rn(v - __bfloat162float(hi));
-                    const int spot = (tid % 64 / 8 ^ (h & 7)) << 4;  // NH is a multiple of 8: the same for lo
-                    *reinterpret_cast<bf16 *>(tile + h * 128 + spot) = hi;
-                    *reinterpret_cast<bf16 *>(tile + (C::NH + h) * 128 + spot) = lo;
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(B(bp_full));
-                // The heads' sums over the warp's positions, halving the heads a lane holds with each exchange.
+                for (int j = 0; j < G16; j++) {
+                    float odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // two sums, for two chains of products
+                    sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
 #pragma unroll
-                for (int w = C::NH / 2, o = 16; w >= 1; w /= 2, o /= 2)
-#pragma unroll
-                    for (int h = 0; h < w; h++) {
-                        const bool up = lane & o;
-                        const float give = up ? part[h] : part[h + w], keep = up ? part[h + w] : part[h];
-                        part[h] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                    for (int s = 0; s < HD / 16; s++) {
+                        uint32_t ka[4];
+                        ldmatrix_x4(ka, ks + own_at<HD>(16 * j + (mi & 1) * 8 + rr, 2 * s + (mi >> 1)));
+                        mma_bf16(s & 1 ? odd : sc[j], ka, qf[s][0], qf[s][1]);
                     }
 #pragma unroll
-                for (int o = 16 / C::NH; o >= 1; o /= 2) part[0] += __shfl_xor_sync(0xffffffffu, part[0], o);
-                {
-                    // The head a lane ends with: bit by bit from the exchanges (lanes that differ below them agree).
-                    int h = 0;
-#pragma unroll
-                    for (int w = C::NH / 2, o = 16; w >= 1; w /= 2, o /= 2) h += lane & o ? w : 0;
-                    sums[warp][h] = part[0];
+                    for (int e = 0; e < 4; e++) sc[j][e] = 16 * j + 8 * (e >> 1) < left ? (sc[j][e] + odd[e]) * scale2 : -INFINITY;
                 }
-                mbar_wait(B(bo_full), n & 1, err, &gave_up);
-                tc_fence_after();
-                uint32_t o[C::NP / 16][16];
+                float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < C::NP / 16; i++) tmem_ld16_nowait(lanes + C::O_COL + 16 * i, o[i]);
-                tmem_wait_ld();
-                tc_fence_before();
-                mbar_arrive(B(bo_read));
-                // O^T: a thread to a dimension (HD = 64: of the warp's KV head), whole lines of a head's partial.
-                const int kv = x.kv + (HD == 64 ? warp / 2 : 0), d = HD == 64 ? tid % 64 : tid, c0 = HD == 64 ? warp / 2 * 8 : 0;
-                const size_t to = ((size_t)x.row * heads + (size_t)kv * group) * pieces + np + x.number;
+                for (int j = 0; j < G16; j++)
 #pragma unroll
-                for (int h = 0; h < 8; h++) {
-                    // Column c0 + h of hi and of lo, c0 0 or 8.
-                    const uint32_t hi = HD == 64 && c0 ? o[0][8 + h] : o[0][h];
-                    const uint32_t lo = HD == 64 ? (c0 ? o[C::NP / 16 - 1][8 + h] : o[C::NP / 16 - 1][h]) : o[0][8 + h];
-                    if (h < group && kv < kvh) out.o[(to + (size_t)h * pieces) * HD + d] = __uint_as_float(hi) + __uint_as_float(lo);
+                    for (int e = 0; e < 4; e++) mx[e & 1] = fmaxf(mx[e & 1], sc[j][e]);
+                // Mostly no score passes its reference by MOVE_PAST, and then nobody need know the maximum.
+                if (__any_sync(0xffffffffu, mx[0] > m[0] + MOVE_PAST || mx[1] > m[1] + MOVE_PAST)) {
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) {
+                        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], x));
+                        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], x));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        if (!(mx[e] > m[e] + MOVE_PAST)) continue;
+                        const float keep = m[e] == -INFINITY ? 0.0f : hw_exp2(m[e] - mx[e]);
+                        m[e] = mx[e];
+                        l[e] *= keep;
+#pragma unroll
+                        for (int j = 0; j < HD / 16; j++) {
+                            o[j][e] *= keep;
+                            o[j][2 + e] *= keep;
+                        }
+                    }
                 }
-                asm volatile("bar.sync 1, 128;" ::: "memory");  // every warp's sums are in
-                if (tid < C::NH) {
-                    const int kv_of = x.kv + tid / 8, h = tid % 8;
-                    const float m = fmaxf(fmaxf(top[0][tid], top[1][tid]), fmaxf(top[2][tid], top[3][tid])) * scale2;
-                    const float l = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
-                    if (h < group && kv_of < kvh)
-                        *reinterpret_cast<float2 *>(out.ml + (((size_t)x.row * heads + (size_t)kv_of * group + h) * pieces + np + x.number) * 2) =
-                            make_float2(m, l);
+                const float nm[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};  // every score -inf: e 0
+#pragma unroll
+                for (int j = 0; j < G16; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        sc[j][e] = hw_exp2(sc[j][e] - nm[e & 1]);
+                        l[e & 1] += sc[j][e];  // the lane's positions' alone
+                    }
+#pragma unroll
+                for (int s = 0; s < G16; s++) {
+                    // e^T as the second operand: each 8 x 8 block turned over among the lanes.
+                    uint32_t h0, h1, l0, l1;
+                    split_pack(sc[s][0], sc[s][1], h0, l0);
+                    split_pack(sc[s][2], sc[s][3], h1, l1);
+                    h0 = turn8(h0);
+                    h1 = turn8(h1);
+                    l0 = turn8(l0);
+                    l1 = turn8(l1);
+#pragma unroll
+                    for (int j = 0; j < HD / 16; j++) {
+                        uint32_t va[4];
+                        ldmatrix_x4_trans(va, vs + own_at<HD>(16 * s + (mi >> 1) * 8 + rr, 2 * j + (mi & 1)));
+                        mma_bf16(o[j], va, h0, h1);
+                        mma_bf16(o[j], va, l0, l1);
+                    }
                 }
             }
-            claims++;
+            __syncwarp();  // the next piece's copies go into the same stages
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+                const int head = 2 * t4 + e;
+                if (head >= group) continue;
+                const size_t to = ((size_t)row * heads + kv * group + head) * pieces + np + piece;
+#pragma unroll
+                for (int j = 0; j < HD / 16; j++) {
+                    out.o[to * HD + 16 * j + g] = o[j][e];
+                    out.o[to * HD + 16 * j + 8 + g] = o[j][2 + e];
+                }
+                if (g == 0) *reinterpret_cast<float2 *>(out.ml + to * 2) = make_float2(m[e], l[e]);
+            }
         }
     }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 4)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"(C::COLS) : "memory");
     pdl_wait();
 }
 
@@ -549,7 +449,7 @@ template <int HD>
 __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
     prefix_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap, tg_params p, const uint32_t *__restrict__ at,
-                  const uint32_t *__restrict__ shared, Partials out, uint32_t pieces, uint32_t box, uint32_t *counter, uint32_t *err) {
+                  const uint32_t *__restrict__ shared, Partials out, uint32_t pieces, uint32_t box, uint32_t *err) {
     using C = Pfx<HD>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -583,6 +483,11 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
         mbar_init(B(bv_clear), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (tid == 32) {
+        prefetch_map(&kmap);
+        prefetch_map(&qmap);
+        prefetch_map(&vmap);
+    }
     // The rows of a Q tile that no query fills (a group that does not divide 128) are zero.
     const int blank = 128 - tile_rows * group;
     auto blank_q = [&](int h, int i0, int step) {
@@ -603,11 +508,6 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     pdl_wait();
-    if (blockIdx.x == 0) {  // own_kernel's counters, before any block of it can start
-        for (uint32_t i = tid; i < own_lists(p.rows); i += C::THREADS) counter[i] = 0;
-        __threadfence();
-        __syncthreads();
-    }
     pdl_launch_dependents();
 
     // A unit: a piece of the prefix, a KV head, NT tiles of queries. The roles walk the block's units each by itself;
@@ -983,30 +883,26 @@ cudaError_t attend(const tg_params &p, const void *q, const void *k, const void 
     cudaError_t e = cudaSuccess;
     if constexpr (sizeof(T) == 2) {
         using C = Pfx<HD>;
-        using W = Own<HD>;
-        const uint32_t group = p.heads / p.kv_heads, tile_rows = 128 / group;
-        const uint32_t box = p.capacity % 128 == 0 ? 128 : p.capacity % 64 == 0 ? 64 : p.capacity % 32 == 0 ? 32 : 16;
-        uint32_t *counter = reinterpret_cast<uint32_t *>(part.ml + items * pieces * 2);
-        CUtensorMap qm, km, vm;
-        if (!map_heads(&km, k, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, box, 1) ||
-            !map_heads(&vm, v, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, box, 1))
-            return cudaErrorInvalidValue;
         if (np) {
-            if (!map_heads(&qm, q, p.heads, p.rows, HD, group, tile_rows)) return cudaErrorInvalidValue;
+            const uint32_t group = p.heads / p.kv_heads, tile_rows = 128 / group;
+            const uint32_t box = p.capacity % 128 == 0 ? 128 : p.capacity % 64 == 0 ? 64 : p.capacity % 32 == 0 ? 32 : 16;
+            CUtensorMap qm, km, vm;
+            if (!map_heads(&qm, q, p.heads, p.rows, HD, group, tile_rows) ||
+                !map_heads(&km, k, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, box, 1) ||
+                !map_heads(&vm, v, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, box, 1))
+                return cudaErrorInvalidValue;
             e = with_smem(prefix_kernel<HD>, C::SMEM);
             if (e != cudaSuccess) return e;
             const uint32_t tiles = (p.rows + tile_rows - 1) / tile_rows, units = np * ((tiles + C::NT - 1) / C::NT) * p.kv_heads;
             e = launch_pdl(prefix_kernel<HD>, dim3(std::min(units, (uint32_t)sm_count)), dim3(C::THREADS), C::SMEM, s, qm, km, vm, p, at,
-                           shared, part, (uint32_t)pieces, box, counter, err);
+                           shared, part, (uint32_t)pieces, box, err);
             if (e != cudaSuccess) return e;
         }
-        if (!map_heads(&qm, q, p.heads, p.rows, HD, group, 1)) return cudaErrorInvalidValue;
-        e = with_smem(own_kernel<HD>, W::SMEM);
+        e = with_smem(own_kernel<HD>, OWN_SMEM);
         if (e != cudaSuccess) return e;
-        const uint64_t most = (uint64_t)p.rows * ((p.kv_heads + W::KVS - 1) / W::KVS) * (pieces - np);
-        if (most > 0xffff0000u) return cudaErrorNotSupported;  // units are counted in 32 bits
-        e = launch_pdl(own_kernel<HD>, dim3((unsigned)std::min<uint64_t>(most, (uint64_t)sm_count * W::BLOCKS)), dim3(OWN_THREADS), W::SMEM, s,
-                       qm, km, vm, p, at, table, part, np, (uint32_t)pieces, box, counter, err);
+        const uint64_t most = ((uint64_t)p.rows * p.kv_heads * (pieces - np) + OWN_WARPS - 1) / OWN_WARPS;
+        e = launch_pdl(own_kernel<HD>, dim3((unsigned)std::min<uint64_t>(most, (uint64_t)sm_count * OWN_BLOCKS)), dim3(OWN_WARPS * 32), OWN_SMEM,
+                       s, p, (const T *)q, (const T *)k, (const T *)v, at, table, part, np, (uint32_t)pieces, err);
     } else {
         e = launch_pdl(pieces_kernel<T, HD>, dim3((unsigned)pieces, p.kv_heads, p.rows), dim3(CHUNK), 0, s, p, (const T *)q, (const T *)k,
                        (const T *)v, at, table, shared, part, np, (uint32_t)pieces, err);
@@ -1018,7 +914,7 @@ cudaError_t attend(const tg_params &p, const void *q, const void *k, const void 
 }  // namespace
 
 uint64_t attention_pages_work(const tg_params &p) {
-    return (uint64_t)p.rows * p.heads * all_pieces(p) * (p.head_dim + 2) * sizeof(float) + own_lists(p.rows) * 4ull + 256;
+    return (uint64_t)p.rows * p.heads * all_pieces(p) * (p.head_dim + 2) * sizeof(float) + 256;
 }
 
 cudaError_t launch_attention_pages(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at,
