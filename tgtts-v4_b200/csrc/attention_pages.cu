@@ -192,12 +192,12 @@ TG_DEVICE uint64_t mn_desc(uint32_t addr, uint32_t chunk) {
 // query heads, at most 8, are the columns of mma.sync.m16n8k16 (S^T = K q^T, O^T = V^T e^T with e split
 // into bf16 hi + lo, against a reference that moves as prefix_kernel's), keys and values gathered from their
 // pages by cp.async, OWN_STAGES - 1 chunks ahead of the products.
-constexpr int OWN_WARPS = 2, OWN_STAGES = 2;
+constexpr int OWN_WARPS = 1, OWN_STAGES = 2;
 constexpr uint32_t OWN_ROWS = 512;  // rows whose pieces are listed at once
 constexpr int own_chunk(int hd) { return 2048 / hd; }
 constexpr int OWN_STAGE = 2 * 2048;  // bf16 of a chunk's keys and values
 constexpr int OWN_SMEM = OWN_WARPS * OWN_STAGES * OWN_STAGE * 2 + (int)OWN_ROWS * 4;
-constexpr int OWN_BLOCKS = 6;  // an SM's, by their shared memory
+constexpr int OWN_BLOCKS = 11;  // an SM's, by their shared memory
 // 16 bytes c of row r of a chunk, as an element: the rows' pieces turned so that eight rows' same piece lie in all banks.
 template <int HD>
 TG_DEVICE int own_at(int r, int c) { return r * HD + ((c ^ (r & 7)) << 3); }
@@ -419,7 +419,8 @@ struct Pfx {
     static constexpr int NT = HD == 64 ? 2 : 1, HALVES = HD / 64, STAGES = HD == 64 ? 3 : 2;
     static constexpr int THREADS = 96 + 128 * NT, SB = HD == 64 ? 1 : 2;
     static constexpr uint32_t HALF = 128 * 64 * 2, TILE = HALF * HALVES;  // 128 rows x 64 dimensions; x HD
-    static constexpr uint32_t Q = 0, K = NT * TILE, V = K + STAGES * TILE, SMEM = V + STAGES * TILE + 1024;
+    static constexpr uint32_t Q = 0, K = NT * TILE, V = K + STAGES * TILE, STAGE = V + STAGES * TILE;  // STAGE: 4 KiB a softmax warp
+    static constexpr uint32_t SMEM = STAGE + NT * 4 * 4096 + 1024;
     static constexpr TG_DEVICE uint32_t s_col(int h, int j) { return NT == 2 ? 256 * h : 128 * (j & 1); }
     static constexpr TG_DEVICE uint32_t p_col(int h) { return NT == 2 ? 256 * h + 128 : 256; }
     static constexpr TG_DEVICE uint32_t o_col(int h) { return NT == 2 ? 256 * h + 192 : 320; }
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
     if (tid == 0) {
         gave_up = 0;
         mbar_init(B(bq_full), 1);
-        mbar_init(B(bq_empty), 4 * C::NT);
+        mbar_init(B(bq_empty), 1);
         for (int i = 0; i < C::STAGES; i++) {
             mbar_init(B(bk_full[i]), 1);
             mbar_init(B(bk_empty[i]), 1);
@@ -490,12 +491,9 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
     }
     // The rows of a Q tile that no query fills (a group that does not divide 128) are zero.
     const int blank = 128 - tile_rows * group;
-    auto blank_q = [&](int h, int i0, int step) {
-        for (int i = i0; i < C::HALVES * blank * 8; i += step)
-            *reinterpret_cast<uint4 *>(smem + C::Q + h * C::TILE + i / (blank * 8) * C::HALF + (tile_rows * group + i / 8 % blank) * 128 + (i % 8) * 16) =
-                make_uint4(0u, 0u, 0u, 0u);
-    };
-    for (int h = 0; h < C::NT; h++) blank_q(h, tid, C::THREADS);
+    for (int i = tid; i < C::NT * C::HALVES * blank * 8; i += C::THREADS)
+        *reinterpret_cast<uint4 *>(smem + C::Q + i / (blank * 8) * C::HALF + (tile_rows * group + i / 8 % blank) * 128 + (i % 8) * 16) =
+            make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
@@ -557,7 +555,7 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
                                 (int)(pos % p.capacity), (int)(id * kvh + x.kv), B(full[b]));
                 id = next;
                 if (warp == 0 && j == 0) {
-                    // Q, once the unit before is done with its own (and with what it staged there).
+                    // Q, once the unit before has all of its S.
                     mbar_wait(B(bq_empty), (done & 1) ^ 1, err, &gave_up);
                     if (lane == 0) {
                         mbar_arrive_expect_tx(B(bq_full), x.nt * C::HALVES * tile_rows * group * 128);
@@ -609,10 +607,15 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
                     tc_fence_after();
                 };
                 mbar_wait(B(bq_full), done & 1, err, &gave_up);
+                // S_j is issued: its keys, and after the last one the queries, may be overwritten once it is done.
+                auto issued_s = [&](int j) {
+                    tc_commit(B(bk_empty[(t0 + j) % C::STAGES]));
+                    if (j == x.n - 1) tc_commit(B(bq_empty));
+                };
                 for (int j = 0; j < C::SB && j < x.n; j++) {
                     wait_k(j);
                     for (int h = 0; h < x.nt; h++) issue_s(j, h);
-                    tc_commit(B(bk_empty[(t0 + j) % C::STAGES]));
+                    issued_s(j);
                 }
                 for (int j = 0; j < x.n; j++) {
                     const int b = (t0 + j) % C::STAGES, next = j + C::SB;  // the S whose buffer S_j leaves free
@@ -624,7 +627,7 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
                         if (C::SB == 1 && next < x.n) {
                             if (h == 0) wait_k(next);
                             issue_s(next, h);
-                            if (h == x.nt - 1) tc_commit(B(bk_empty[(t0 + next) % C::STAGES]));
+                            if (h == x.nt - 1) issued_s(next);
                         }
                         if (h == 0) {
                             mbar_wait(B(bv_full[b]), ((t0 + j) / C::STAGES) & 1, err, &gave_up);
@@ -641,7 +644,7 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
                     if (C::SB == 2 && next < x.n) {
                         wait_k(next);
                         issue_s(next, 0);
-                        tc_commit(B(bk_empty[(t0 + next) % C::STAGES]));
+                        issued_s(next);
                     }
                 }
                 t0 += x.n;
@@ -675,19 +678,8 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
                 for (int j = 0; j < x.n; j++, t++) {
                     mbar_wait(B(bs_full[h * C::SB + (C::SB - 1) * (t & 1)]), (t / C::SB) & 1, err, &gave_up);
                     tc_fence_after();
-                    if (j == 0) {  // no reference yet: the tile's maximum first
-                        float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll 1
-                        for (int c = 0; c < 128; c += 64) {
-                            float sv[64];
-                            scores(0, c, sv);
-#pragma unroll
-                            for (int i = 0; i < 64; i += 2) mx[(i / 2) % 2] = max3(mx[(i / 2) % 2], sv[i], sv[i + 1]);
-                        }
-                        mref = fmaxf(mx[0], mx[1]) * scale2;
-                    }
                     // P_j against mref into TMEM with its sum, the tile's raw maximum alongside; P_j takes P_{j-1}'s place once
-                    // PV_{j-1} has read it. Where the maximum has passed a reference by MOVE_PAST, O (with PV_{j-1} in it) is
+                    // PV_{j-1} has read it. (The first tile's first half of keys gives the first reference.) Where the maximum has passed a reference by MOVE_PAST, O (with PV_{j-1} in it) is
                     // rescaled, a query that keeps its reference times 1, and the warp's pass runs again from S_j.
                     float a = 1.0f, sum;
                     for (bool again = false;; again = true) {
@@ -695,12 +687,19 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
 #pragma unroll
                         for (int i = 0; i < 4; i++) sums[i] = make_float2(0.0f, 0.0f);
                         float mx[2] = {-INFINITY, -INFINITY};
-                        const float nm = mref != -INFINITY ? -mref : -INFINITY;  // every score -inf: P comes out 0
-                        const float2 scale22 = make_float2(scale2, scale2), neg_m = make_float2(nm, nm);
+                        const float2 scale22 = make_float2(scale2, scale2);
 #pragma unroll
                         for (int c = 0; c < 128; c += 64) {
                             float sv[64];
                             scores(j, c, sv);
+                            if (c == 0 && j == 0 && !again) {
+                                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                                for (int i = 0; i < 64; i += 2) top[(i / 2) % 4] = max3(top[(i / 2) % 4], sv[i], sv[i + 1]);
+                                mref = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                            }
+                            const float nm = mref != -INFINITY ? -mref : -INFINITY;  // every score -inf: P comes out 0
+                            const float2 neg_m = make_float2(nm, nm);
                             uint32_t pk[2][16];
 #pragma unroll
                             for (int i = 0; i < 64; i += 2) {
@@ -725,7 +724,7 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
                         if (move) mref = m_tile;
                         tmem_wait_st();
 #pragma unroll 1
-                        for (int c = 0; c < HD; c += 16) {
+                        for (int c = 0; c < HD && j > 0; c += 16) {
                             uint32_t o[16];
                             tmem_ld16_nowait(lanes + C::o_col(h) + c, o);
                             tmem_wait_ld();
@@ -742,43 +741,45 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
                 }
                 mbar_wait(B(bo_full[h]), (t - 1) & 1, err, &gave_up);
                 tc_fence_after();
-                // The partials, where a query is one: O as it stands in TMEM by way of shared memory (the Q tile: every S
-                // of the unit is done once its last PV is), so that a store covers whole lines of four queries;
-                // references and sums. A row of the stage is 32 values, its 16-byte pieces turned by the row.
+                // The partials, where a query is one: O as it stands in TMEM by way of shared memory, so that a store covers
+                // whole lines of four queries; references and sums. A row of the stage is 32 values, its 16-byte pieces
+                // turned by the row.
                 const int row = (x.tile0 + h) * tile_rows + m / group;
                 const bool real = m < tile_rows * group && row < (int)p.rows;
                 const uint64_t to = real ? ((uint64_t)row * heads + x.kv * group + m % group) * pieces + x.piece : ~0ull;
-                float4 *stage = reinterpret_cast<float4 *>(smem + C::Q + h * C::TILE + quad * 4096);
-#pragma unroll 1
+                float4 *stage = reinterpret_cast<float4 *>(smem + C::STAGE + (warp - 2) * 4096);
+                float4 *dst[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const uint64_t q = __shfl_sync(0xffffffffu, to, 4 * i + lane / 8);
+                    dst[i] = q != ~0ull ? reinterpret_cast<float4 *>(out.o + q * HD) + lane % 8 : nullptr;
+                }
+                uint32_t o[2][16];
+                tmem_ld16_nowait(lanes + C::o_col(h), o[0]);
+                tmem_ld16_nowait(lanes + C::o_col(h) + 16, o[1]);
+#pragma unroll
                 for (int c = 0; c < HD; c += 32) {
-                    uint32_t o[2][16];
-                    tmem_ld16_nowait(lanes + C::o_col(h) + c, o[0]);
-                    tmem_ld16_nowait(lanes + C::o_col(h) + c + 16, o[1]);
                     tmem_wait_ld();
 #pragma unroll
                     for (int e = 0; e < 8; e++)
                         stage[lane * 8 + (e ^ (lane & 7))] =
                             make_float4(__uint_as_float(o[e / 4][e % 4 * 4]), __uint_as_float(o[e / 4][e % 4 * 4 + 1]),
                                         __uint_as_float(o[e / 4][e % 4 * 4 + 2]), __uint_as_float(o[e / 4][e % 4 * 4 + 3]));
+                    if (c + 32 < HD) {
+                        tmem_ld16_nowait(lanes + C::o_col(h) + c + 32, o[0]);
+                        tmem_ld16_nowait(lanes + C::o_col(h) + c + 48, o[1]);
+                    }
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int q = 4 * i + lane / 8;
-                        const uint64_t dst = __shfl_sync(0xffffffffu, to, q);
-                        if (dst != ~0ull) *reinterpret_cast<float4 *>(out.o + dst * HD + c + 4 * (lane % 8)) = stage[q * 8 + (lane % 8 ^ (q & 7))];
+                        if (dst[i]) dst[i][c / 4] = stage[q * 8 + (lane % 8 ^ (q & 7))];
                     }
                     __syncwarp();
                 }
                 if (real) *reinterpret_cast<float2 *>(out.ml + to * 2) = make_float2(mref, l);
                 tc_fence_before();
-                if (blank) {  // as Q expects it, once every warp of the tile is done with its part of the stage
-                    asm volatile("bar.sync %0, 128;" ::"r"(1 + h) : "memory");
-                    blank_q(h, m, 128);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next Q's copies
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(B(bq_empty));
         }
     }
     tc_fence_before();
@@ -872,6 +873,14 @@ bool map_heads(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t outer,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Opts a kernel into its shared memory with all of an SM's as shared memory, so that blocks of the kernels that run
+// beside it find room there.
+template <typename F>
+cudaError_t with_all_smem(F kernel, size_t bytes) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+}
+
 template <typename T, int HD>
 cudaError_t attend(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at, const uint32_t *table,
                    const uint32_t *shared, void *work, void *out, uint32_t *err, int sm_count, cudaStream_t s) {
@@ -891,14 +900,14 @@ cudaError_t attend(const tg_params &p, const void *q, const void *k, const void 
                 !map_heads(&km, k, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, box, 1) ||
                 !map_heads(&vm, v, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, box, 1))
                 return cudaErrorInvalidValue;
-            e = with_smem(prefix_kernel<HD>, C::SMEM);
+            e = with_all_smem(prefix_kernel<HD>, C::SMEM);
             if (e != cudaSuccess) return e;
             const uint32_t tiles = (p.rows + tile_rows - 1) / tile_rows, units = np * ((tiles + C::NT - 1) / C::NT) * p.kv_heads;
             e = launch_pdl(prefix_kernel<HD>, dim3(std::min(units, (uint32_t)sm_count)), dim3(C::THREADS), C::SMEM, s, qm, km, vm, p, at,
                            shared, part, (uint32_t)pieces, box, err);
             if (e != cudaSuccess) return e;
         }
-        e = with_smem(own_kernel<HD>, OWN_SMEM);
+        e = with_all_smem(own_kernel<HD>, OWN_SMEM);
         if (e != cudaSuccess) return e;
         const uint64_t most = ((uint64_t)p.rows * p.kv_heads * (pieces - np) + OWN_WARPS - 1) / OWN_WARPS;
         e = launch_pdl(own_kernel<HD>, dim3((unsigned)std::min<uint64_t>(most, (uint64_t)sm_count * OWN_BLOCKS)), dim3(OWN_WARPS * 32), OWN_SMEM,
