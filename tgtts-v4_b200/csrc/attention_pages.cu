@@ -38,6 +38,7 @@ __host__ __device__ inline uint64_t all_pieces(const tg_params &p) {
 struct Partials {
     float *o, *ml;
 };
+constexpr uint32_t OWN_ROWS = 512;  // rows whose own pieces are listed at once
 
 // A row's own length and request; false for a row that computes nothing.
 TG_DEVICE bool paged_row(const tg_params &p, const uint32_t *at, int row, uint32_t &length, uint32_t &seq, uint32_t *err) {
@@ -193,7 +194,6 @@ TG_DEVICE uint64_t mn_desc(uint32_t addr, uint32_t chunk) {
 // into bf16 hi + lo, against a reference that moves as prefix_kernel's), keys and values gathered from their
 // pages by cp.async, OWN_STAGES - 1 chunks ahead of the products.
 constexpr int OWN_WARPS = 1, OWN_STAGES = 2;
-constexpr uint32_t OWN_ROWS = 512;  // rows whose pieces are listed at once
 constexpr int own_chunk(int hd) { return 2048 / hd; }
 constexpr int OWN_STAGE = 2 * 2048;  // bf16 of a chunk's keys and values
 constexpr int OWN_SMEM = OWN_WARPS * OWN_STAGES * OWN_STAGE * 2 + (int)OWN_ROWS * 4;
@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
     __shared__ uint32_t total_s;
     constexpr int CH = own_chunk(HD), VECS = HD / 8, G16 = CH / 16, ROWS = 32 / VECS;
     // Behind prefix_kernel this one starts under it: that kernel lets it go once what comes before both has
-    // ended (its own wait), and the two share nothing. A block still waits before it ends, for the join.
+    // ended (its own wait), and the two share nothing. One block waits for it all the same before it ends, so that
+    // the join waits for both; the others make room for the next.
     if (np == 0) pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3, mi = lane >> 3, rr = lane & 7;
@@ -395,29 +396,33 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
             }
         }
     }
-    pdl_wait();
+    if (blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 // ---- shared pieces, bf16 ------------------------------------------------------------------------------
 // A block an SM, over units of a piece, a KV head and NT tiles of up to 128 queries, query m of a tile being
-// head m % group of row m / group of the tile's rows, against the piece's keys in tiles of 128. Eleven warps (seven for one tile):
-//   warps 0 and the last  TMA: Q and the K tiles, and the V tiles, page by page (boxes of the largest of
+// head m % group of row m / group of the tile's rows, against the piece's keys in tiles of 128. Twelve warps (eight for one tile; warp 3 has no part):
+//   warps 0 and 2  TMA: Q and the K tiles, and the V tiles, page by page (boxes of the largest of
 //              128, 64, 32 and 16 positions that divides a page) into STAGES stages of
 //              128-byte-swizzled halves of 64 dimensions; values past the prefix in its last tile set to
 //              zero (0 x NaN is NaN). Two warps, as a copy's issue takes about 110 clocks: 16 to a tile
 //              of K or V for pages of 16 (8 KiB of HD = 128 each);
 //   warp 1     TMEM and the MMAs: S_j = Q K_j^T (M = 128, N = 128), O += P_j V_j (N = HD; P in TMEM, V
 //              read MN-major), the tile's next S ahead of its PV so that the softmax runs under it;
-//   warps 2-5  (and 6-9)  the softmax of a tile, a thread to a query: P_j = 2^(S_j scale - mref) as bf16
+//   warps 4-7  (and 8-11)  the softmax of a tile, a thread to a query: P_j = 2^(S_j scale - mref) as bf16
 //              into TMEM against a reference that moves only when a tile's maximum passes it by 2^8 (O
 //              then rescaled in place), the same pass as the prefill's attention kernel.
 // HD = 64: two tiles, which share the keys' copies, each with S, P and O in 256 columns. HD = 128: one tile
 // with two S buffers (S 2 x 128, P 64, O 128), as two tiles do not fit TMEM's 512 columns.
+// The softmax warps take registers from the first four (setmaxnreg), so that own_kernel's blocks find room beside.
 // Every wait is bounded (the context's error word, then the block runs out).
 template <int HD>
 struct Pfx {
     static constexpr int NT = HD == 64 ? 2 : 1, HALVES = HD / 64, STAGES = HD == 64 ? 3 : 2;
-    static constexpr int THREADS = 96 + 128 * NT, SB = HD == 64 ? 1 : 2;
+    static constexpr int THREADS = 128 + 128 * NT, SB = HD == 64 ? 1 : 2;
+    // Registers a thread: at launch, of warps 0-3 and of the softmax warps (the same sum).
+    static constexpr int REGS = HD == 64 ? 136 : 144, FEW = 72, MANY = HD == 64 ? 168 : 216;
+    static_assert(FEW + NT * MANY == (1 + NT) * REGS, "setmaxnreg draws on the launch's registers");
     static constexpr uint32_t HALF = 128 * 64 * 2, TILE = HALF * HALVES;  // 128 rows x 64 dimensions; x HD
     static constexpr uint32_t Q = 0, K = NT * TILE, V = K + STAGES * TILE, STAGE = V + STAGES * TILE;  // STAGE: 4 KiB a softmax warp
     static constexpr uint32_t SMEM = STAGE + NT * 4 * 4096 + 1024;
@@ -447,7 +452,7 @@ TG_DEVICE float max3(float a, float b, float c) {
     return d;
 }
 template <int HD>
-__global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
+__global__ void __launch_bounds__(Pfx<HD>::THREADS) __maxnreg__(Pfx<HD>::REGS)
     prefix_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap, tg_params p, const uint32_t *__restrict__ at,
                   const uint32_t *__restrict__ shared, Partials out, uint32_t pieces, uint32_t box, uint32_t *err) {
@@ -525,134 +530,138 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
         x.n = (int)((x.keys + 127) / 128);
         return x;
     };
-    const bool values = warp == C::THREADS / 32 - 1;
-    if (warp == 0 || values) {
-        // A lane to a copy: one half of the dimensions, one box of positions; the pages' numbers a tile ahead.
-        const int boxes = 128 / (int)box, seg = lane % boxes, half = lane / boxes;
-        uint64_t *full = values ? bv_full : bk_full, *empty = values ? bv_empty : bk_empty;
-        const CUtensorMap *map = values ? &vmap : &kmap;
-        int t = 0, done = 0, last_clear = -1;  // last_clear: the tile whose values were last cleared
-        for (uint32_t u = blockIdx.x; u < units; u += gridDim.x, done++) {
-            const Unit x = unit(u);
-            auto page_of = [&](int j) {
-                const uint32_t in = j * 128 + seg * box;
-                uint32_t id = in < x.keys ? __ldg(shared + (x.begin + in) / p.capacity) : 0u;
-                if (id >= p.slots) {
-                    atomicExch(err, ERR_BAD_INDEX);
-                    id = 0;
-                }
-                return id;
-            };
-            uint32_t id = page_of(0);
-            for (int j = 0; j < x.n; j++, t++) {
-                const int b = t % C::STAGES, live = min(128, (int)x.keys - j * 128), segs = (live + (int)box - 1) / (int)box;
-                const uint32_t pos = x.begin + j * 128 + seg * box, next = page_of(j + 1);
-                mbar_wait(B(empty[b]), ((t / C::STAGES) & 1) ^ 1, err, &gave_up);
-                if (lane == 0) mbar_arrive_expect_tx(B(full[b]), C::HALVES * segs * box * 128);
-                __syncwarp();
-                if (half < C::HALVES && seg < segs)
-                    tma_load_3d(base + (values ? C::V : C::K) + b * C::TILE + half * C::HALF + seg * box * 128, map, half * 64,
-                                (int)(pos % p.capacity), (int)(id * kvh + x.kv), B(full[b]));
-                id = next;
-                if (warp == 0 && j == 0) {
-                    // Q, once the unit before has all of its S.
-                    mbar_wait(B(bq_empty), (done & 1) ^ 1, err, &gave_up);
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(B(bq_full), x.nt * C::HALVES * tile_rows * group * 128);
-                        for (int h = 0; h < x.nt; h++)
-                            for (int c = 0; c < C::HALVES; c++)
-                                tma_load_3d(base + C::Q + h * C::TILE + c * C::HALF, &qmap, c * 64, x.kv * group, (x.tile0 + h) * tile_rows, B(bq_full));
-                    }
-                    __syncwarp();
-                }
-            }
-            if (values && x.keys % 128) {
-                const int b = (t - 1) % C::STAGES, keep = (int)(x.keys % 128);
-                mbar_wait(B(bv_full[b]), ((t - 1) / C::STAGES) & 1, err, &gave_up);
-                // The clear before has been used: its stage's next copy waited for that, or else this does.
-                if (last_clear >= 0 && t - 1 < last_clear + C::STAGES)
-                    mbar_wait(B(bv_empty[last_clear % C::STAGES]), (last_clear / C::STAGES) & 1, err, &gave_up);
-                last_clear = t - 1;
-                uint8_t *vt = smem + C::V + b * C::TILE;
-                for (int i = lane; i < C::HALVES * (128 - keep) * 8; i += 32) {
-                    const int c = i / ((128 - keep) * 8), r = keep + i / 8 % (128 - keep);  // a swizzled row is 128 whole bytes
-                    *reinterpret_cast<uint4 *>(vt + c * C::HALF + r * 128 + (i % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // for the tensor cores' reads
-                __syncwarp();
-                if (lane == 0) mbar_arrive(B(bv_clear));
-            }
-        }
-        // Every copy has landed before the block can end.
-        for (int i = t > C::STAGES ? t - C::STAGES : 0; i < t; i++) mbar_wait(B(full[i % C::STAGES]), (i / C::STAGES) & 1, err, &gave_up);
-        if (warp == 0) mbar_wait(B(bq_full), (done - 1) & 1, err, &gave_up);
-    } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc_s = bf16_idesc(128, 128);
-            constexpr uint32_t idesc_o = bf16_idesc(128, HD) | (1u << 16);  // B (V) MN-major
-            int t0 = 0, done = 0, cleared = 0, seen[2] = {0, 0};  // seen: the tiles of keys each tile of queries has had
+    const bool values = warp == 2;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEW));
+        if (warp == 0 || values) {
+            // A lane to a copy: one half of the dimensions, one box of positions; the pages' numbers a tile ahead.
+            const int boxes = 128 / (int)box, seg = lane % boxes, half = lane / boxes;
+            uint64_t *full = values ? bv_full : bk_full, *empty = values ? bv_empty : bk_empty;
+            const CUtensorMap *map = values ? &vmap : &kmap;
+            int t = 0, done = 0, last_clear = -1;  // last_clear: the tile whose values were last cleared
             for (uint32_t u = blockIdx.x; u < units; u += gridDim.x, done++) {
                 const Unit x = unit(u);
-                auto issue_s = [&](int j, int h) {
-                    const uint32_t kt = base + C::K + ((t0 + j) % C::STAGES) * C::TILE, qt = base + C::Q + h * C::TILE;
-                    const int at_s = seen[h] + j;
-#pragma unroll
-                    for (int i = 0; i < HD / 16; i++)
-                        tc_mma(tmem + C::s_col(h, at_s), sw128_desc(qt + (i / 4) * C::HALF + (i % 4) * 32),
-                               sw128_desc(kt + (i / 4) * C::HALF + (i % 4) * 32), idesc_s, i > 0 ? 1u : 0u);
-                    tc_commit(B(bs_full[h * C::SB + (C::SB - 1) * (at_s & 1)]));
+                auto page_of = [&](int j) {
+                    const uint32_t in = j * 128 + seg * box;
+                    uint32_t id = in < x.keys ? __ldg(shared + (x.begin + in) / p.capacity) : 0u;
+                    if (id >= p.slots) {
+                        atomicExch(err, ERR_BAD_INDEX);
+                        id = 0;
+                    }
+                    return id;
                 };
-                auto wait_k = [&](int j) {
-                    mbar_wait(B(bk_full[(t0 + j) % C::STAGES]), ((t0 + j) / C::STAGES) & 1, err, &gave_up);
-                    tc_fence_after();
-                };
-                mbar_wait(B(bq_full), done & 1, err, &gave_up);
-                // S_j is issued: its keys, and after the last one the queries, may be overwritten once it is done.
-                auto issued_s = [&](int j) {
-                    tc_commit(B(bk_empty[(t0 + j) % C::STAGES]));
-                    if (j == x.n - 1) tc_commit(B(bq_empty));
-                };
-                for (int j = 0; j < C::SB && j < x.n; j++) {
-                    wait_k(j);
-                    for (int h = 0; h < x.nt; h++) issue_s(j, h);
-                    issued_s(j);
+                uint32_t id = page_of(0);
+                for (int j = 0; j < x.n; j++, t++) {
+                    const int b = t % C::STAGES, live = min(128, (int)x.keys - j * 128), segs = (live + (int)box - 1) / (int)box;
+                    const uint32_t pos = x.begin + j * 128 + seg * box, next = page_of(j + 1);
+                    mbar_wait(B(empty[b]), ((t / C::STAGES) & 1) ^ 1, err, &gave_up);
+                    if (lane == 0) mbar_arrive_expect_tx(B(full[b]), C::HALVES * segs * box * 128);
+                    __syncwarp();
+                    if (half < C::HALVES && seg < segs)
+                        tma_load_3d(base + (values ? C::V : C::K) + b * C::TILE + half * C::HALF + seg * box * 128, map, half * 64,
+                                    (int)(pos % p.capacity), (int)(id * kvh + x.kv), B(full[b]));
+                    id = next;
+                    if (warp == 0 && j == 0) {
+                        // Q, once the unit before has all of its S.
+                        mbar_wait(B(bq_empty), (done & 1) ^ 1, err, &gave_up);
+                        if (lane == 0) {
+                            mbar_arrive_expect_tx(B(bq_full), x.nt * C::HALVES * tile_rows * group * 128);
+                            for (int h = 0; h < x.nt; h++)
+                                for (int c = 0; c < C::HALVES; c++)
+                                    tma_load_3d(base + C::Q + h * C::TILE + c * C::HALF, &qmap, c * 64, x.kv * group, (x.tile0 + h) * tile_rows, B(bq_full));
+                        }
+                        __syncwarp();
+                    }
                 }
-                for (int j = 0; j < x.n; j++) {
-                    const int b = (t0 + j) % C::STAGES, next = j + C::SB;  // the S whose buffer S_j leaves free
-                    const uint32_t v = base + C::V + b * C::TILE;
-                    for (int h = 0; h < x.nt; h++) {
-                        // P_j in TMEM, S_j read, and O rescaled to the query's reference (or the unit's before stored).
-                        mbar_wait(B(bp_full[h]), (seen[h] + j) & 1, err, &gave_up);
+                if (values && x.keys % 128) {
+                    const int b = (t - 1) % C::STAGES, keep = (int)(x.keys % 128);
+                    mbar_wait(B(bv_full[b]), ((t - 1) / C::STAGES) & 1, err, &gave_up);
+                    // The clear before has been used: its stage's next copy waited for that, or else this does.
+                    if (last_clear >= 0 && t - 1 < last_clear + C::STAGES)
+                        mbar_wait(B(bv_empty[last_clear % C::STAGES]), (last_clear / C::STAGES) & 1, err, &gave_up);
+                    last_clear = t - 1;
+                    uint8_t *vt = smem + C::V + b * C::TILE;
+                    for (int i = lane; i < C::HALVES * (128 - keep) * 8; i += 32) {
+                        const int c = i / ((128 - keep) * 8), r = keep + i / 8 % (128 - keep);  // a swizzled row is 128 whole bytes
+                        *reinterpret_cast<uint4 *>(vt + c * C::HALF + r * 128 + (i % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // for the tensor cores' reads
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(B(bv_clear));
+                }
+            }
+            // Every copy has landed before the block can end.
+            for (int i = t > C::STAGES ? t - C::STAGES : 0; i < t; i++) mbar_wait(B(full[i % C::STAGES]), (i / C::STAGES) & 1, err, &gave_up);
+            if (warp == 0) mbar_wait(B(bq_full), (done - 1) & 1, err, &gave_up);
+        } else if (warp == 1) {
+            if (lane == 0) {
+                constexpr uint32_t idesc_s = bf16_idesc(128, 128);
+                constexpr uint32_t idesc_o = bf16_idesc(128, HD) | (1u << 16);  // B (V) MN-major
+                int t0 = 0, done = 0, cleared = 0, seen[2] = {0, 0};  // seen: the tiles of keys each tile of queries has had
+                for (uint32_t u = blockIdx.x; u < units; u += gridDim.x, done++) {
+                    const Unit x = unit(u);
+                    auto issue_s = [&](int j, int h) {
+                        const uint32_t kt = base + C::K + ((t0 + j) % C::STAGES) * C::TILE, qt = base + C::Q + h * C::TILE;
+                        const int at_s = seen[h] + j;
+#pragma unroll
+                        for (int i = 0; i < HD / 16; i++)
+                            tc_mma(tmem + C::s_col(h, at_s), sw128_desc(qt + (i / 4) * C::HALF + (i % 4) * 32),
+                                   sw128_desc(kt + (i / 4) * C::HALF + (i % 4) * 32), idesc_s, i > 0 ? 1u : 0u);
+                        tc_commit(B(bs_full[h * C::SB + (C::SB - 1) * (at_s & 1)]));
+                    };
+                    auto wait_k = [&](int j) {
+                        mbar_wait(B(bk_full[(t0 + j) % C::STAGES]), ((t0 + j) / C::STAGES) & 1, err, &gave_up);
                         tc_fence_after();
-                        if (C::SB == 1 && next < x.n) {
-                            if (h == 0) wait_k(next);
-                            issue_s(next, h);
-                            if (h == x.nt - 1) issued_s(next);
-                        }
-                        if (h == 0) {
-                            mbar_wait(B(bv_full[b]), ((t0 + j) / C::STAGES) & 1, err, &gave_up);
-                            if (j == x.n - 1 && x.keys % 128) mbar_wait(B(bv_clear), cleared++ & 1, err, &gave_up);
+                    };
+                    mbar_wait(B(bq_full), done & 1, err, &gave_up);
+                    // S_j is issued: its keys, and after the last one the queries, may be overwritten once it is done.
+                    auto issued_s = [&](int j) {
+                        tc_commit(B(bk_empty[(t0 + j) % C::STAGES]));
+                        if (j == x.n - 1) tc_commit(B(bq_empty));
+                    };
+                    for (int j = 0; j < C::SB && j < x.n; j++) {
+                        wait_k(j);
+                        for (int h = 0; h < x.nt; h++) issue_s(j, h);
+                        issued_s(j);
+                    }
+                    for (int j = 0; j < x.n; j++) {
+                        const int b = (t0 + j) % C::STAGES, next = j + C::SB;  // the S whose buffer S_j leaves free
+                        const uint32_t v = base + C::V + b * C::TILE;
+                        for (int h = 0; h < x.nt; h++) {
+                            // P_j in TMEM, S_j read, and O rescaled to the query's reference (or the unit's before stored).
+                            mbar_wait(B(bp_full[h]), (seen[h] + j) & 1, err, &gave_up);
                             tc_fence_after();
-                        }
+                            if (C::SB == 1 && next < x.n) {
+                                if (h == 0) wait_k(next);
+                                issue_s(next, h);
+                                if (h == x.nt - 1) issued_s(next);
+                            }
+                            if (h == 0) {
+                                mbar_wait(B(bv_full[b]), ((t0 + j) / C::STAGES) & 1, err, &gave_up);
+                                if (j == x.n - 1 && x.keys % 128) mbar_wait(B(bv_clear), cleared++ & 1, err, &gave_up);
+                                tc_fence_after();
+                            }
 #pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            tc_mma_ts(tmem + C::o_col(h), tmem + C::p_col(h) + 8 * i, mn_desc(v + i * 2048, C::HALF), idesc_o,
-                                      (j > 0 || i > 0) ? 1u : 0u);
-                        tc_commit(B(bo_full[h]));
+                            for (int i = 0; i < 8; i++)
+                                tc_mma_ts(tmem + C::o_col(h), tmem + C::p_col(h) + 8 * i, mn_desc(v + i * 2048, C::HALF), idesc_o,
+                                          (j > 0 || i > 0) ? 1u : 0u);
+                            tc_commit(B(bo_full[h]));
+                        }
+                        tc_commit(B(bv_empty[b]));
+                        if (C::SB == 2 && next < x.n) {
+                            wait_k(next);
+                            issue_s(next, 0);
+                            issued_s(next);
+                        }
                     }
-                    tc_commit(B(bv_empty[b]));
-                    if (C::SB == 2 && next < x.n) {
-                        wait_k(next);
-                        issue_s(next, 0);
-                        issued_s(next);
-                    }
+                    t0 += x.n;
+                    for (int h = 0; h < x.nt; h++) seen[h] += x.n;
                 }
-                t0 += x.n;
-                for (int h = 0; h < x.nt; h++) seen[h] += x.n;
             }
         }
     } else {
-        const int h = (warp - 2) / 4, quad = warp & 3, m = quad * 32 + lane;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::MANY));
+        const int h = warp / 4 - 1, quad = warp & 3, m = quad * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         const float scale2 = 1.4426950408889634f / sqrtf((float)HD);  // log2(e) / sqrt(hd)
         int t = 0;  // the tiles of keys this tile of queries has had
@@ -747,7 +756,7 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS, 1)
                 const int row = (x.tile0 + h) * tile_rows + m / group;
                 const bool real = m < tile_rows * group && row < (int)p.rows;
                 const uint64_t to = real ? ((uint64_t)row * heads + x.kv * group + m % group) * pieces + x.piece : ~0ull;
-                float4 *stage = reinterpret_cast<float4 *>(smem + C::STAGE + (warp - 2) * 4096);
+                float4 *stage = reinterpret_cast<float4 *>(smem + C::STAGE + (warp - 4) * 4096);
                 float4 *dst[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
@@ -902,6 +911,12 @@ cudaError_t attend(const tg_params &p, const void *q, const void *k, const void 
                 return cudaErrorInvalidValue;
             e = with_all_smem(prefix_kernel<HD>, C::SMEM);
             if (e != cudaSuccess) return e;
+            // Its setmaxnreg counts on the launch's registers: fewer would be waited for without end.
+            static const int regs = [] {
+                cudaFuncAttributes a;
+                return cudaFuncGetAttributes(&a, prefix_kernel<HD>) == cudaSuccess ? a.numRegs : 0;
+            }();
+            if (regs != C::REGS) return cudaErrorInvalidConfiguration;
             const uint32_t tiles = (p.rows + tile_rows - 1) / tile_rows, units = np * ((tiles + C::NT - 1) / C::NT) * p.kv_heads;
             e = launch_pdl(prefix_kernel<HD>, dim3(std::min(units, (uint32_t)sm_count)), dim3(C::THREADS), C::SMEM, s, qm, km, vm, p, at,
                            shared, part, (uint32_t)pieces, box, err);
