@@ -311,12 +311,16 @@ typedef struct {
 /* Context::dispatch (crates/vulkan/src/context.rs:520): runs one dispatch, waits, and gives its
  * GPU time in ns (may be NULL). */
 int tg_dispatch_once(tg_ctx *ctx, const tg_dispatch *d, double *ns);
-/* The same dispatch, with the same checks, enqueued on a stream of the caller's (a cudaStream_t of the
- * context's device; NULL: the legacy stream; TG_ECUDA for another device's) without waiting; it allocates nothing, so it may be
- * captured into the caller's CUDA graph. The buffers have to live until the work is done, and
- * what the kernels report in the context's error word comes with the next tg_ctx_synchronize after
- * that. */
-int tg_dispatch_enqueue(tg_ctx *ctx, const tg_dispatch *d, void *stream);
+/* A dispatch for callers with streams of their own: resolved and checked once, as a program's, then
+ * enqueued as often as needed on any stream of the context's device (a cudaStream_t; NULL: the legacy
+ * stream; TG_ECUDA for another device's), without waiting. An enqueue allocates nothing and may be
+ * captured into the caller's CUDA graph. The buffers have to live until the work is done; what the
+ * kernels report in the context's error word comes with the next tg_ctx_synchronize after that. One
+ * call may be enqueued from several threads, or on several streams, where the work itself may overlap. */
+typedef struct tg_call tg_call;
+int tg_call_create(tg_ctx *ctx, const tg_dispatch *d, tg_call **out);
+int tg_call_enqueue(const tg_call *call, void *stream);
+int tg_call_destroy(tg_call *call);
 /* What a dispatch's checks ask of its bindings, without a device: the bytes each binding of `kernel`
  * must hold for these params, in order, into `bytes` (room for n; may be NULL when n is 0), their number
  * into *count. Refuses what tg_dispatch_once refuses of the params (TG_EINVAL, TG_ESHAPE). */

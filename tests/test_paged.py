@@ -93,7 +93,9 @@ def test_unknown_kernels_and_null_handles(pkg):
     for kernel in (13, 31, 1008):
         assert pkg.library().tg_dispatch_needs(kernel, ctypes.byref(plan(pkg)), None, 0, ctypes.byref(count)) == 1
     assert pkg.library().tg_dispatch_needs(27, None, None, 0, ctypes.byref(count)) == 1
-    assert pkg.library().tg_dispatch_enqueue(None, None, None) == 1
+    assert pkg.library().tg_call_enqueue(None, None) == 1
+    assert pkg.library().tg_call_create(None, None, None) == 1
+    assert pkg.library().tg_call_destroy(None) == 0
     out = ctypes.c_void_p()
     assert pkg.library().tg_mem_wrap(None, 16, 16, ctypes.byref(out)) == 1
 

@@ -173,7 +173,9 @@ SIGNATURES = {
     "tg_mem_fill": (_I, [_P, _U64, _U32, _U64]),
     "tg_copy_regions": (_I, [_P, _P, _P, ctypes.POINTER(TgRegion), _SZ]),
     "tg_dispatch_once": (_I, [_P, ctypes.POINTER(TgDispatch), _DP]),
-    "tg_dispatch_enqueue": (_I, [_P, _P, _P]),
+    "tg_call_create": (_I, [_P, ctypes.POINTER(TgDispatch), ctypes.POINTER(_P)]),
+    "tg_call_enqueue": (_I, [_P, _P]),
+    "tg_call_destroy": (_I, [_P]),
     "tg_dispatch_needs": (_I, [_U32, ctypes.POINTER(TgParams), ctypes.POINTER(_U64), _SZ, ctypes.POINTER(_SZ)]),
     "tg_program_create": (_I, [_P, ctypes.POINTER(TgDispatch), _SZ, _I, ctypes.POINTER(_P)]),
     "tg_program_destroy": (_I, [_P]),
@@ -566,31 +568,39 @@ def dispatch_once(ctx: Context, kernel: str, p: TgParams,
 
 
 class Dispatch:
-    """One kernel-table dispatch, made once and enqueued as often as needed, on any stream of the
-    context's device, without waiting (tg_dispatch_enqueue; inside a CUDA graph capture too).
-    `bindings` are buffers (the whole of each) or (buffer, offset, bytes). `params` may be changed
-    between calls: each is checked against the bindings' sizes."""
+    """One kernel-table dispatch, checked once and enqueued as often as needed, on any stream of the
+    context's device, without waiting (tg_call; inside a CUDA graph capture too). `bindings` are
+    buffers (the whole of each, kept alive) or (buffer, offset, bytes)."""
 
     def __init__(self, ctx: Context, kernel: str, p: TgParams, bindings, label: str = ""):
+        self.handle = None
         if kernel not in KERNELS:
             raise InvalidError(f"no kernel {kernel!r}")
         parts = [b if isinstance(b, tuple) else (b, 0, b.nbytes) for b in bindings]
-        self.ctx, self.kernel, self.params = ctx, kernel, p
-        self._keep = ([m for m, _, _ in parts], label.encode() or None,
-                      (TgBinding * len(parts))(*[TgBinding(m.handle, o, n) for m, o, n in parts]))
-        self._c = TgDispatch(KERNELS[kernel], ctypes.pointer(p), self._keep[2], len(parts), self._keep[1])
-        self._at = ctypes.addressof(self._c)
-        self._enqueue = library().tg_dispatch_enqueue
+        b = (TgBinding * len(parts))(*[TgBinding(m.handle, o, n) for m, o, n in parts])
+        d = TgDispatch(KERNELS[kernel], ctypes.pointer(p), b, len(parts), label.encode())
+        h = ctypes.c_void_p()
+        check(library().tg_call_create(ctx.handle, ctypes.byref(d), ctypes.byref(h)))
+        self.ctx, self.memories = ctx, [m for m, _, _ in parts]
+        self.handle, self._enqueue = h, library().tg_call_enqueue
 
     def enqueue(self, stream: int = 0) -> None:
         """Runs it on `stream` (a cudaStream_t as an integer, 0 the legacy stream; `ctx.stream` the
         context's own), in that stream's order."""
-        for m in self._keep[0]:
-            if not m.handle:
-                raise InvalidError(f"{self.kernel}: a buffer that was freed")
-        status = self._enqueue(self.ctx.handle, self._at, stream)
+        status = self._enqueue(self.handle, stream)
         if status:
             check(status)
+
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            library().tg_call_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def needs(kernel: str, p: TgParams) -> list[int]:

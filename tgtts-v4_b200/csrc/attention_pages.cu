@@ -891,48 +891,63 @@ cudaError_t with_all_smem(F kernel, size_t bytes) {
 }
 
 template <typename T, int HD>
-cudaError_t attend(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at, const uint32_t *table,
-                   const uint32_t *shared, void *work, void *out, uint32_t *err, int sm_count, cudaStream_t s) {
-    const uint64_t pieces = all_pieces(p), items = (uint64_t)p.rows * p.heads;
-    if (pieces > 0x7fffffffu || p.kv_heads > 65535) return cudaErrorNotSupported;
+cudaError_t attend(const tg_params &p, const void *q_, const void *k_, const void *v_, const uint32_t *at, const uint32_t *table,
+                   const uint32_t *shared, void *work, void *out_, uint32_t *err, int sm_count, Enqueue &run) {
+    const uint64_t all = all_pieces(p), items = (uint64_t)p.rows * p.heads;
+    if (all > 0x7fffffffu || p.kv_heads > 65535) return cudaErrorNotSupported;
+    const T *q = static_cast<const T *>(q_), *k = static_cast<const T *>(k_), *v = static_cast<const T *>(v_);
+    T *out = static_cast<T *>(out_);
     float *o = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(work) + 255) & ~uintptr_t(255));
-    Partials part{o, o + items * pieces * HD};
-    const uint32_t np = shared_pieces(p.first);
-    cudaError_t e = cudaSuccess;
-    if constexpr (sizeof(T) == 2) {
+    const Partials part{o, o + items * all * HD};
+    const uint32_t np = shared_pieces(p.first), pieces = (uint32_t)all;
+    auto join = [=](cudaStream_t s) {
+        return launch_pdl(join_kernel<T, HD>, dim3((unsigned)items), dim3(JOIN_THREADS), 0, s, p, at, part, np, pieces, out);
+    };
+    if constexpr (sizeof(T) == 4) {
+        run = [=](cudaStream_t s) {
+            const cudaError_t e = launch_pdl(pieces_kernel<T, HD>, dim3(pieces, p.kv_heads, p.rows), dim3(CHUNK), 0, s, p, q, k, v, at, table,
+                                             shared, part, np, pieces, err);
+            return e != cudaSuccess ? e : join(s);
+        };
+    } else {
         using C = Pfx<HD>;
-        if (np) {
-            const uint32_t group = p.heads / p.kv_heads, tile_rows = 128 / group;
-            const uint32_t box = p.capacity % 128 == 0 ? 128 : p.capacity % 64 == 0 ? 64 : p.capacity % 32 == 0 ? 32 : 16;
-            CUtensorMap qm, km, vm;
-            if (!map_heads(&qm, q, p.heads, p.rows, HD, group, tile_rows) ||
-                !map_heads(&km, k, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, box, 1) ||
-                !map_heads(&vm, v, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, box, 1))
-                return cudaErrorInvalidValue;
-            e = with_all_smem(prefix_kernel<HD>, C::SMEM);
-            if (e != cudaSuccess) return e;
-            // Its setmaxnreg counts on the launch's registers: fewer would be waited for without end.
-            static const int regs = [] {
-                cudaFuncAttributes a;
-                return cudaFuncGetAttributes(&a, prefix_kernel<HD>) == cudaSuccess ? a.numRegs : 0;
-            }();
-            if (regs != C::REGS) return cudaErrorInvalidConfiguration;
-            const uint32_t tiles = (p.rows + tile_rows - 1) / tile_rows, units = np * ((tiles + C::NT - 1) / C::NT) * p.kv_heads;
-            e = launch_pdl(prefix_kernel<HD>, dim3(std::min(units, (uint32_t)sm_count)), dim3(C::THREADS), C::SMEM, s, qm, km, vm, p, at,
-                           shared, part, (uint32_t)pieces, box, err);
-            if (e != cudaSuccess) return e;
-        }
-        e = with_all_smem(own_kernel<HD>, OWN_SMEM);
+        cudaError_t e = with_all_smem(own_kernel<HD>, OWN_SMEM);
         if (e != cudaSuccess) return e;
         const uint64_t most = ((uint64_t)p.rows * p.kv_heads * (pieces - np) + OWN_WARPS - 1) / OWN_WARPS;
-        e = launch_pdl(own_kernel<HD>, dim3((unsigned)std::min<uint64_t>(most, (uint64_t)sm_count * OWN_BLOCKS)), dim3(OWN_WARPS * 32), OWN_SMEM,
-                       s, p, (const T *)q, (const T *)k, (const T *)v, at, table, part, np, (uint32_t)pieces, err);
-    } else {
-        e = launch_pdl(pieces_kernel<T, HD>, dim3((unsigned)pieces, p.kv_heads, p.rows), dim3(CHUNK), 0, s, p, (const T *)q, (const T *)k,
-                       (const T *)v, at, table, shared, part, np, (uint32_t)pieces, err);
+        const unsigned own_blocks = (unsigned)std::min<uint64_t>(most, (uint64_t)sm_count * OWN_BLOCKS);
+        auto own = [=](cudaStream_t s) {
+            const cudaError_t e = launch_pdl(own_kernel<HD>, dim3(own_blocks), dim3(OWN_WARPS * 32), OWN_SMEM, s, p, q, k, v, at, table, part, np,
+                                             pieces, err);
+            return e != cudaSuccess ? e : join(s);
+        };
+        if (np == 0) {
+            run = own;
+            return cudaSuccess;
+        }
+        const uint32_t group = p.heads / p.kv_heads, tile_rows = 128 / group;
+        const uint32_t box = p.capacity % 128 == 0 ? 128 : p.capacity % 64 == 0 ? 64 : p.capacity % 32 == 0 ? 32 : 16;
+        CUtensorMap qm, km, vm;
+        if (!map_heads(&qm, q, p.heads, p.rows, HD, group, tile_rows) ||
+            !map_heads(&km, k, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, box, 1) ||
+            !map_heads(&vm, v, p.capacity, (uint64_t)p.slots * p.kv_heads, HD, box, 1))
+            return cudaErrorInvalidValue;
+        e = with_all_smem(prefix_kernel<HD>, C::SMEM);
+        if (e != cudaSuccess) return e;
+        // Its setmaxnreg counts on the launch's registers: fewer would be waited for without end.
+        cudaFuncAttributes a;
+        e = cudaFuncGetAttributes(&a, prefix_kernel<HD>);
+        if (e != cudaSuccess) return e;
+        if (a.numRegs != C::REGS) return cudaErrorInvalidConfiguration;
+        const uint64_t tiles = (p.rows + tile_rows - 1) / tile_rows, units = np * ((tiles + C::NT - 1) / C::NT) * p.kv_heads;
+        if (units > 0x7fffffffu) return cudaErrorNotSupported;
+        const unsigned blocks = (unsigned)std::min<uint64_t>(units, (uint64_t)sm_count);
+        run = [=](cudaStream_t s) {
+            const cudaError_t e = launch_pdl(prefix_kernel<HD>, dim3(blocks), dim3(C::THREADS), C::SMEM, s, qm, km, vm, p, at, shared, part, pieces,
+                                             box, err);
+            return e != cudaSuccess ? e : own(s);
+        };
     }
-    if (e != cudaSuccess) return e;
-    return launch_pdl(join_kernel<T, HD>, dim3((unsigned)items), dim3(JOIN_THREADS), 0, s, p, at, part, np, (uint32_t)pieces, (T *)out);
+    return cudaSuccess;
 }
 
 }  // namespace
@@ -941,14 +956,14 @@ uint64_t attention_pages_work(const tg_params &p) {
     return (uint64_t)p.rows * p.heads * all_pieces(p) * (p.head_dim + 2) * sizeof(float) + 256;
 }
 
-cudaError_t launch_attention_pages(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at,
-                                   const uint32_t *table, const uint32_t *shared, void *work, void *out, uint32_t *err,
-                                   int sm_count, cudaStream_t s) {
+cudaError_t make_attention_pages(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at,
+                                 const uint32_t *table, const uint32_t *shared, void *work, void *out, uint32_t *err,
+                                 int sm_count, Enqueue &run) {
     if (p.dtype == TG_BF16)
-        return p.head_dim == 64 ? attend<bf16, 64>(p, q, k, v, at, table, shared, work, out, err, sm_count, s)
-                                : attend<bf16, 128>(p, q, k, v, at, table, shared, work, out, err, sm_count, s);
-    return p.head_dim == 64 ? attend<float, 64>(p, q, k, v, at, table, shared, work, out, err, sm_count, s)
-                            : attend<float, 128>(p, q, k, v, at, table, shared, work, out, err, sm_count, s);
+        return p.head_dim == 64 ? attend<bf16, 64>(p, q, k, v, at, table, shared, work, out, err, sm_count, run)
+                                : attend<bf16, 128>(p, q, k, v, at, table, shared, work, out, err, sm_count, run);
+    return p.head_dim == 64 ? attend<float, 64>(p, q, k, v, at, table, shared, work, out, err, sm_count, run)
+                            : attend<float, 128>(p, q, k, v, at, table, shared, work, out, err, sm_count, run);
 }
 
 }  // namespace tg

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <algorithm>
 #include <cstring>
+#include <memory>
 #include <new>
 #include <thread>
 
@@ -519,7 +520,12 @@ int enqueue_launch(const Launch &l, uint32_t *err, cudaStream_t s, int sm_count)
         case TG_KERNEL_DIT_EULER: e = launch_dit_euler(p, b[0], b[1], b[2], F(3), F(4), s); break;
         case TG_KERNEL_PAGE_PLAN: e = launch_page_plan(p, U(0), U(1), U(2), U(3), U(4), U(5), U(6), U(7), U(8), err, s); break;
         case TG_KERNEL_ROPE_PAGES: e = launch_rope_pages(p, U(0), U(1), b[2], F(3), F(4), b[5], b[6], b[7], err, s); break;
-        case TG_KERNEL_ATTENTION_PAGES: e = launch_attention_pages(p, b[0], b[1], b[2], U(3), U(4), U(5), b[6], b[7], err, sm_count, s); break;
+        case TG_KERNEL_ATTENTION_PAGES: {
+            Enqueue once;
+            if (!l.ready) e = make_attention_pages(p, b[0], b[1], b[2], U(3), U(4), U(5), b[6], b[7], err, sm_count, once);
+            if (e == cudaSuccess) e = l.ready ? l.ready(s) : once(s);
+            break;
+        }
         case TG_KERNEL_LOGITS_PICK: e = launch_logits_pick(p, b[0], U(1), U(2), F(3), U(4), F(5), U(6), b[7], U(8), err, s); break;
         default: return fail(TG_EINVAL, "no kernel %u", l.kernel);
     }
@@ -528,6 +534,15 @@ int enqueue_launch(const Launch &l, uint32_t *err, cudaStream_t s, int sm_count)
                     l.kernel == KERNEL_DECODE_STEP ? "decode_step" : kernel_name(table_kernel(l.kernel)), l.label.c_str(),
                     cudaGetErrorString(e));
     return TG_OK;
+}
+
+int prepare_launch(Launch &l, uint32_t *err, int sm_count) {
+    if (l.kernel != TG_KERNEL_ATTENTION_PAGES) return TG_OK;
+    void *const *b = l.ptr.data();
+    auto U = [&](int i) { return static_cast<uint32_t *>(b[i]); };
+    const cudaError_t e = make_attention_pages(l.p, b[0], b[1], b[2], U(3), U(4), U(5), b[6], b[7], err, sm_count, l.ready);
+    if (e == cudaSuccess) return TG_OK;
+    return fail(e == cudaErrorNotSupported ? TG_ESHAPE : TG_ECUDA, "preparing attention_pages: %s", cudaGetErrorString(e));
 }
 
 // ---- programs ------------------------------------------------------------------------------------
@@ -906,23 +921,42 @@ struct DeviceGuard {
 };
 }  // namespace
 
-extern "C" int tg_dispatch_enqueue(tg_ctx *ctx, const tg_dispatch *d, void *stream) try {
-    if (!ctx || !d) return fail(TG_EINVAL, "tg_dispatch_enqueue: null argument");
-    Launch l;
-    int st = resolve(*d, l);
-    if (!st) st = check_launch(l);
+struct tg_call {
+    tg_ctx *ctx;
+    Launch launch;
+};
+
+extern "C" int tg_call_create(tg_ctx *ctx, const tg_dispatch *d, tg_call **out) try {
+    if (!ctx || !d || !out) return fail(TG_EINVAL, "tg_call_create: null argument");
+    *out = nullptr;
+    std::unique_ptr<tg_call> call(new tg_call{ctx, {}});
+    int st = resolve(*d, call->launch);
+    if (!st) st = check_launch(call->launch);
     if (st) return st;
     for (uint32_t i = 0; i < d->n_bindings; i++)
         if (d->bindings[i].mem->ctx->device != ctx->device)
-            return fail(TG_EINVAL, "tg_dispatch_enqueue: binding %u is on device %d, the context on %d", i,
+            return fail(TG_EINVAL, "tg_call_create: binding %u is on device %d, the context on %d", i,
                         d->bindings[i].mem->ctx->device, ctx->device);
+    const DeviceGuard guard(ctx->device);
+    st = prepare_launch(call->launch, ctx->err_dev, ctx->sm_count);
+    if (st) return st;
+    *out = call.release();
+    return TG_OK;
+} catch (const std::bad_alloc &) {
+    return TG_ENOMEM;  // host memory; no message, which would need some too
+}
+
+extern "C" int tg_call_enqueue(const tg_call *call, void *stream) {
+    if (!call) return fail(TG_EINVAL, "null call");
     // A stream of another device than the current one refuses the launch itself (cudaStreamGetDevice
     // would say so first, but not while the stream is being captured).
-    const DeviceGuard guard(ctx->device);
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return enqueue_launch(l, ctx->err_dev, s, ctx->sm_count);
-} catch (const std::bad_alloc &) {
-    return TG_ENOMEM;  // host memory for the dispatch's bindings; no message, which would need some too
+    const DeviceGuard guard(call->ctx->device);
+    return enqueue_launch(call->launch, call->ctx->err_dev, static_cast<cudaStream_t>(stream), call->ctx->sm_count);
+}
+
+extern "C" int tg_call_destroy(tg_call *call) {
+    delete call;
+    return TG_OK;
 }
 
 extern "C" int tg_dispatch_needs(uint32_t kernel, const tg_params *p, uint64_t *bytes, size_t n, size_t *count) try {

@@ -6,6 +6,7 @@
 
 #include <cstdarg>
 #include <cstdint>
+#include <functional>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -101,6 +102,9 @@ cudaError_t launch_attention_split_join(const tg_params &p, const void *q, const
 // Decoders of at least this many rows run their projections on tcgen05 (every bucket of them).
 constexpr uint32_t DTC_MIN_ROWS = 16;
 
+// Enqueues a prepared dispatch's kernels on a stream.
+using Enqueue = std::function<cudaError_t(cudaStream_t)>;
+
 // One dispatch resolved to device pointers, as the kernel table launches it.
 struct Launch {
     uint32_t kernel = 0;
@@ -109,12 +113,15 @@ struct Launch {
     std::vector<uint64_t> bytes;
     std::string label;
     DecodeStep step{};  // KERNEL_DECODE_STEP only
+    Enqueue ready{};    // prepare_launch's, for a dispatch that is enqueued many times
 };
 
 // The kernel table: checks a dispatch's params against its bindings' sizes (what each binding
 // must hold for the grid the params give), then launches it on `stream`.
 int check_launch(const Launch &l);
 int enqueue_launch(const Launch &l, uint32_t *err_dev, cudaStream_t stream, int sm_count);
+// Makes what a checked launch's enqueues share, where it has something.
+int prepare_launch(Launch &l, uint32_t *err_dev, int sm_count);
 
 // A captured chain of launches (a CUDA graph) with optional events between them.
 struct Program {
@@ -243,9 +250,10 @@ cudaError_t launch_page_plan(const tg_params &p, const uint32_t *held, const uin
 cudaError_t launch_rope_pages(const tg_params &p, const uint32_t *at, const uint32_t *place, const void *c,
                               const float *cosv, const float *sinv, void *q, void *k, void *v, uint32_t *err,
                               cudaStream_t s);
-cudaError_t launch_attention_pages(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at,
-                                   const uint32_t *table, const uint32_t *shared, void *work, void *out, uint32_t *err,
-                                   int sm_count, cudaStream_t s);
+// Its launches, with the copies' descriptors and the kernels' attributes made once.
+cudaError_t make_attention_pages(const tg_params &p, const void *q, const void *k, const void *v, const uint32_t *at,
+                                 const uint32_t *table, const uint32_t *shared, void *work, void *out, uint32_t *err,
+                                 int sm_count, Enqueue &run);
 uint64_t attention_pages_work(const tg_params &p);
 cudaError_t launch_logits_pick(const tg_params &p, const void *logits, const uint32_t *seen, const uint32_t *spans,
                                const float *penalties, const uint32_t *bias_ids, const float *bias,
