@@ -193,52 +193,60 @@ TG_DEVICE bool rope_row(const tg_params &p, uint32_t pos, uint32_t to, uint32_t 
     return true;
 }
 
-// For a rotated part that is a multiple of 8: eight dimensions of two heads of a row to a thread (heads h
-// and h + half the heads, which turn by the same angles), rotated ones as four pairs (in the half layout
-// two runs of four, each a warp's whole sectors). All of a thread's loads of c leave before the first is
-// used, and before it knows whether its row is spare. A block takes ROPE_ROWS x the row's threads.
+// For a rotated part that is a multiple of 8: a thread takes eight dimensions of two heads (h and h + half the heads,
+// which turn by the same angles), rotated ones as four pairs (in the half layout two runs of four, each a warp's
+// whole sectors), of every gridDim-th group of rows: where they lie in a row is worked out once. All of a
+// row's loads of c leave before it is known whether the row is spare.
 constexpr int ROPE_THREADS = 256;
 
-template <typename T, typename C, bool INTER>
+template <typename T, typename C, bool INTER, int HD>
 __global__ void __launch_bounds__(ROPE_THREADS)
-    rope_pages_kernel(tg_params p, Divisor page, Divisor row_units, uint32_t block_rows, const uint32_t *__restrict__ at,
-                      const uint32_t *__restrict__ place, const C *__restrict__ c, const float *__restrict__ cosv,
-                      const float *__restrict__ sinv, T *__restrict__ q, T *__restrict__ k, T *__restrict__ v, uint32_t *err) {
+    rope_pages_kernel(tg_params p, Divisor page, uint32_t units, uint32_t row_units, uint32_t block_rows,
+                      const uint32_t *__restrict__ at, const uint32_t *__restrict__ place, const C *__restrict__ c,
+                      const float *__restrict__ cosv, const float *__restrict__ sinv, T *__restrict__ q, T *__restrict__ k,
+                      T *__restrict__ v, uint32_t *err) {
+    // A block's `units` threads of a row, from unit blockIdx.y x units on, times block_rows rows.
+    const uint32_t heads = p.heads + 2 * p.kv_heads, apart = (heads + 1) / 2, half = p.k / 2;
+    const uint32_t sub = threadIdx.x / units, unit = blockIdx.y * units + threadIdx.x % units;
+    const uint32_t head0 = unit / (HD / 8), head1 = head0 + apart, u = unit % (HD / 8);
+    const bool here[2] = {unit < row_units, unit < row_units && head1 < heads};
+    const bool rotated = p.rope && u < p.k / 8;
+    const bool turned[2] = {rotated && head0 < p.heads + p.kv_heads, rotated && head1 < p.heads + p.kv_heads};
+    uint32_t d0[2], d1[2];
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+        d0[n] = (turned[n] && !INTER) ? 4 * u : 8 * u;
+        d1[n] = (turned[n] && !INTER) ? half + 4 * u : 8 * u + 4;
+    }
+    const C *x[2] = {c + (size_t)head0 * HD, c + (size_t)head1 * HD};
+    const size_t row_values = (size_t)heads * HD;
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t units = p.head_dim / 8, heads = p.heads + 2 * p.kv_heads, apart = (heads + 1) / 2;
-    const uint32_t row0 = blockIdx.x * block_rows, here = min(block_rows, p.rows - row0) * row_units.d;
-    for (uint32_t i = threadIdx.x; i < here; i += ROPE_THREADS) {
-        const uint32_t in_block = row_units.div(i), row = row0 + in_block, in_row = i - in_block * row_units.d;
-        const uint32_t u = in_row % units, head0 = in_row / units, head1 = head0 + apart;  // units: 8 or 16
-        const uint32_t pos = at[row], to = place[row];
-        const bool rotated = p.rope && u < p.k / 8;
+    const uint32_t step = gridDim.x * block_rows;
+    for (uint32_t row = blockIdx.x * block_rows + sub; row < p.rows; row += step) {
         float4 a[2], b[2];
-        uint32_t d0[2], d1[2];
-        bool turned[2];
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-            const uint32_t head = n ? head1 : head0;
-            turned[n] = rotated && head < p.heads + p.kv_heads;
-            d0[n] = (turned[n] && !INTER) ? 4 * u : 8 * u;
-            d1[n] = (turned[n] && !INTER) ? p.k / 2 + 4 * u : 8 * u + 4;
-            if (head >= heads) continue;
-            const C *x = c + ((size_t)row * heads + head) * p.head_dim;
-            a[n] = load4(x + d0[n]);
-            b[n] = load4(x + d1[n]);
+            if (!here[n]) continue;
+            a[n] = load4(x[n] + row * row_values + d0[n]);
+            b[n] = load4(x[n] + row * row_values + d1[n]);
         }
+        const uint32_t pos = at[row], to = place[row];
         if (!rope_row(p, pos, to, err)) continue;
+        const uint32_t id = page.div(to), off = to - id * p.capacity;
         float4 co, si;
         if (turned[0] || turned[1]) {
-            co = __ldg(reinterpret_cast<const float4 *>(cosv + (size_t)pos * (p.k / 2)) + u);
-            si = __ldg(reinterpret_cast<const float4 *>(sinv + (size_t)pos * (p.k / 2)) + u);
+            co = __ldg(reinterpret_cast<const float4 *>(cosv + (size_t)pos * half) + u);
+            si = __ldg(reinterpret_cast<const float4 *>(sinv + (size_t)pos * half) + u);
         }
 #pragma unroll
         for (int n = 0; n < 2; n++) {
             const uint32_t head = n ? head1 : head0;
-            if (head >= heads) continue;
-            T *o = rope_out(p, page, row, head, to, q, k, v);
-            if (!o) continue;
+            if (!here[n] || (head >= p.heads && to == SPARE)) continue;
+            const bool value = head >= p.heads + p.kv_heads;
+            T *o = head < p.heads
+                       ? q + ((size_t)row * p.heads + head) * HD
+                       : (value ? v : k) + (((size_t)id * p.kv_heads + (head - p.heads - (value ? p.kv_heads : 0))) * p.capacity + off) * HD;
             if (turned[n]) {
                 if (INTER) {
                     turn(a[n].x, a[n].y, co.x, si.x);
@@ -561,16 +569,25 @@ cudaError_t pick_t(const tg_params &p, const void *logits, const uint32_t *seen,
 template <typename T, typename C>
 cudaError_t rope_t(const tg_params &p, const uint32_t *at, const uint32_t *place, const void *c, const float *cs,
                    const float *sn, void *q, void *k, void *v, uint32_t *err, cudaStream_t s) {
-    const bool wide = p.k % 8 == 0;
-    const uint32_t heads = p.heads + 2 * p.kv_heads, units = wide ? (heads + 1) / 2 * (p.head_dim / 8) : heads * (p.head_dim / 2);
-    const uint32_t block_rows = units >= ROPE_THREADS ? 1 : ROPE_THREADS / units;
-    const dim3 grid((p.rows + block_rows - 1) / block_rows);
+    const uint32_t heads = p.heads + 2 * p.kv_heads;
+    const Divisor page(p.capacity);
+    if (p.k % 8) {
+        const uint32_t units = heads * (p.head_dim / 2), block_rows = units >= ROPE_THREADS ? 1 : ROPE_THREADS / units;
+        return launch_pdl(rope_pages_any_kernel<T, C>, dim3((p.rows + block_rows - 1) / block_rows), dim3(ROPE_THREADS), 0, s, p, page,
+                          Divisor(units), block_rows, at, place, (const C *)c, cs, sn, (T *)q, (T *)k, (T *)v, err);
+    }
+    // A row's units over gridDim.y blocks of about equal width; as many rows to a block as fit; no more blocks than
+    // four waves of four an SM (more rows to a thread then: 45.7 us for 32768 rows of 20 heads of 64; sixteen waves or a
+    // thread a row 47.3 and 51.3, one wave 52.1).
+    const uint32_t row_units = (heads + 1) / 2 * (p.head_dim / 8), ny = (row_units + ROPE_THREADS - 1) / ROPE_THREADS;
+    const uint32_t units = (row_units + ny - 1) / ny, block_rows = ROPE_THREADS / units;
+    const uint32_t nx = min((p.rows + block_rows - 1) / block_rows, 4u * 4 * 148 / ny + 1);
     auto run = [&](auto kern) {
-        return launch_pdl(kern, grid, dim3(ROPE_THREADS), 0, s, p, Divisor(p.capacity), Divisor(units), block_rows, at, place,
-                          (const C *)c, cs, sn, (T *)q, (T *)k, (T *)v, err);
+        return launch_pdl(kern, dim3(nx, ny), dim3(units * block_rows), 0, s, p, page, units, row_units, block_rows, at, place, (const C *)c, cs, sn,
+                          (T *)q, (T *)k, (T *)v, err);
     };
-    if (!wide) return run(rope_pages_any_kernel<T, C>);
-    return p.flags & 1 ? run(rope_pages_kernel<T, C, true>) : run(rope_pages_kernel<T, C, false>);
+    if (p.head_dim == 64) return p.flags & 1 ? run(rope_pages_kernel<T, C, true, 64>) : run(rope_pages_kernel<T, C, false, 64>);
+    return p.flags & 1 ? run(rope_pages_kernel<T, C, true, 128>) : run(rope_pages_kernel<T, C, false, 128>);
 }
 
 }  // namespace
