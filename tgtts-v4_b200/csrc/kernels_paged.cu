@@ -373,13 +373,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
                 if (t + VEC <= n) raw[j] = __ldcs(reinterpret_cast<const Raw *>(x + t));
             }
         };
-        // With controls to count first, the run's tiles come into L2 meanwhile (register loads would stand before the
-        // history's in the memory pipe).
         if (!controls) load(l0);
-        else if (VEC > 1)
-            for (uint32_t l = l0 + tid * PICK_TILE; l < min(end, l0 + PICK_AHEAD); l += PICK_THREADS * PICK_TILE)
-                if (token_of(l) + PICK_TILE <= n)
-                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x + token_of(l)), "n"(PICK_TILE * sizeof(T)) : "memory");
         auto allow = [&](uint32_t t) { return bits ? __ldg(bits + t / 32) >> (t % 32) : 0xffffffffu; };
         auto hits = [&](uint32_t in) { return controls ? touched[in / 32] >> (in % 32) & ALL : 0u; };
         if (controls) {
@@ -400,6 +394,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
                     if (in < end - l0) in_biases(in, i);
                 }
             };
+            constexpr uint32_t LINE = 128 / sizeof(T);
             constexpr uint32_t W = PICK_RUN / 32 / PICK_THREADS;  // words of the bit map to a thread
             uint32_t total, upto, marks[W];
             while (true) {
@@ -411,6 +406,10 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
                     if (!(touched[in / 32] >> (in % 32) & 1)) atomicOr(touched + in / 32, 1u << (in % 32));
                 };
                 entries(touch, touch);
+                // The history is here: while it is counted the run's first logits come into L2. (Before it, their traffic
+                // held it up.)
+                for (uint32_t l = l0 + tid * LINE; l < min(end, l0 + PICK_AHEAD); l += PICK_THREADS * LINE)
+                    if (token_of(l) < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + token_of(l)) : "memory");
                 __syncthreads();
                 uint32_t sum = 0;
 #pragma unroll
