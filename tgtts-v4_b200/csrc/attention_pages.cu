@@ -8,7 +8,7 @@
 // For bf16 the shared pieces run on tcgen05 (prefix_kernel): the rows of all requests, times the query
 // heads of one KV head, are the 128 rows of its products, so that a tile of keys and values is read
 // once for 128 queries. The own pieces, which no other row shares, run on mma.sync
-// (own_kernel), bound by the caches' bytes. f32 runs on the CUDA cores (pieces_kernel).
+// (own_kernel), bound by the caches' bytes. f32 runs on the CUDA cores (f32_kernel, for both kinds of piece).
 #include <algorithm>
 
 #include "mma_common.cuh"
@@ -19,14 +19,13 @@ namespace tg {
 namespace {
 
 constexpr uint32_t SPARE = TG_SPARE;
-constexpr int CHUNK = 128;  // positions a block takes at once
 
 // Own positions of a piece.
 constexpr uint32_t OWN_PIECE = 128;
-// Shared positions of a piece: at most 16 pieces, each whole chunks.
+// Shared positions of a piece: at most 16 pieces, each whole tiles of 128.
 __host__ __device__ inline uint32_t shared_piece(uint32_t first) {
     const uint32_t even = (first + 15) / 16;
-    return even <= CHUNK ? CHUNK : (even + CHUNK - 1) / CHUNK * CHUNK;
+    return even <= 128 ? 128 : (even + 127) / 128 * 128;
 }
 __host__ __device__ inline uint32_t shared_pieces(uint32_t first) { return (first + shared_piece(first) - 1) / shared_piece(first); }
 __host__ __device__ inline uint64_t all_pieces(const tg_params &p) {
@@ -53,117 +52,147 @@ TG_DEVICE bool paged_row(const tg_params &p, const uint32_t *at, int row, uint32
     return true;
 }
 
-// A piece of a row for one KV head, on the CUDA cores: a thread to a position for the scores, to a
-// dimension for the output, chunk by chunk with a running maximum.
-template <typename T, int HD>
-__global__ void __launch_bounds__(CHUNK)
-    pieces_kernel(tg_params p, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-                  const uint32_t *__restrict__ at, const uint32_t *__restrict__ table, const uint32_t *__restrict__ shared,
-                  Partials out, uint32_t np, uint32_t pieces, uint32_t *err) {
-    constexpr int G = MAX_GROUP, HALVES = CHUNK / HD;
-    __shared__ __align__(16) float qs[G][HD];
-    __shared__ float es[G][CHUNK], red[G][CHUNK / 32], mrun[G], lrun[G], alpha[G];
-    __shared__ uint64_t from[CHUNK];
-    __shared__ float add[HALVES > 1 ? G : 1][HD];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.z, kv = blockIdx.y, piece = blockIdx.x;
-    const int heads = p.heads, kvh = p.kv_heads, group = heads / kvh;
-    uint32_t length, seq;
-    if (!paged_row(p, at, row, length, seq, kv == 0 && piece == 0 && tid == 0 ? err : nullptr)) return;
-    const bool own = piece >= (int)np;
-    const uint32_t size = own ? OWN_PIECE : shared_piece(p.first), n = own ? length : p.first;
-    const uint64_t begin = (uint64_t)(own ? piece - np : piece) * size;
-    if (begin >= n) return;
-    const uint32_t stop = (uint32_t)min((uint64_t)n, begin + size);
-    const uint32_t *list = own ? table + (size_t)seq * p.stride : shared;
+// ---- f32, on the CUDA cores ----------------------------------------------------------------------------
+// A block to a piece for one KV head and up to QN queries: of a row's own positions for the heads of the row, of
+// the shared prefix for the heads of as many rows as fit, so that its keys and values are read once for them.
+// Chunks of keys in shared memory (32 KB of them, and of values); a thread to a key and a share of the queries for
+// the scores, to a dimension and a share of the queries for the output, with a running maximum over the chunks.
+// Products, sums and statistics in f32; the references are natural.
+// Bound by the shared memory reads that feed the multiply-adds (three of 16 bytes to 32 of those). One launch for
+// both kinds of piece: two cost 5 us more in a call of 10 rows. 32 queries a block against one row's heads:
+// 128 rows of 16 heads over 2 at head dim 64 behind 4096 shared positions in 119 us against 211, 18 TFLOP/s.
+constexpr int F32_THREADS = 256, F32_QUERIES = 32;
+template <int HD, int QN>
+struct F32 {
+    static constexpr int CHUNK = 8192 / HD;  // keys at once
+    static constexpr int KROW = HD + 4;  // floats of a key: eight keys' same 16 bytes lie in all banks
+    static constexpr int V = CHUNK * KROW, Q = V + CHUNK * HD, E = Q + QN * HD, SMEM = (E + QN * CHUNK) * 4;
+};
+
+template <int HD, int QN, bool SHARED>
+__device__ __forceinline__ void f32_piece(const tg_params &p, const float *__restrict__ q, const float *__restrict__ k,
+                                          const float *__restrict__ v, const uint32_t *__restrict__ at, const uint32_t *__restrict__ table,
+                                          const uint32_t *__restrict__ shared, const Partials &out, uint32_t index, uint32_t kv, uint32_t tile,
+                                          uint32_t np, uint32_t pieces, uint32_t *err) {
+    using C = F32<HD, QN>;
+    constexpr int CHUNK = C::CHUNK, PARTS = F32_THREADS / HD, QH = QN * CHUNK / F32_THREADS, QP = QN / PARTS;
+    static_assert(QH >= 1 && QP >= 1 && QN % PARTS == 0, "threads");
+    extern __shared__ __align__(16) float f32_mem[];
+    float *ks = f32_mem, *vs = f32_mem + C::V, *qs = f32_mem + C::Q, *es = f32_mem + C::E;
+    __shared__ float mrun[QN], lrun[QN], keep_s[QN];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, heads = p.heads, kvh = p.kv_heads, group = heads / kvh;
+    const int rows = SHARED ? QN / group : 1, row0 = tile * rows, queries = min(rows, (int)p.rows - row0) * group;
+    uint32_t length = p.first, seq = 0;
+    const uint32_t size = SHARED ? shared_piece(p.first) : OWN_PIECE;
+    const uint64_t begin = (uint64_t)index * size;
+    if ((!SHARED && !paged_row(p, at, row0, length, seq, kv == 0 && index == 0 && tid == 0 ? err : nullptr)) || begin >= length) return;
+    const uint32_t stop = (uint32_t)min((uint64_t)length, begin + size);
+    const uint32_t *list = SHARED ? shared : table + (size_t)seq * p.stride;
     const float scale = 1.0f / sqrtf((float)HD);
-    for (int i = tid; i < group * HD; i += CHUNK) qs[i / HD][i % HD] = to_f32<T>(q[((size_t)row * heads + kv * group) * HD + i]) * scale;
-    if (tid < G) {
+    auto head_of = [&](int j) { return ((size_t)(row0 + j / group) * heads + (size_t)kv * group + j % group); };
+    for (int i = tid; i < QN * (HD / 4); i += F32_THREADS) {
+        const int j = i / (HD / 4), d = i % (HD / 4) * 4;
+        float4 x = j < queries ? *reinterpret_cast<const float4 *>(q + head_of(j) * HD + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        *reinterpret_cast<float4 *>(qs + j * HD + d) = make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
+    }
+    if (tid < QN) {
         mrun[tid] = -INFINITY;
         lrun[tid] = 0.0f;
     }
-    float acc[G];
+    float acc[QP];
 #pragma unroll
-    for (int g = 0; g < G; g++) acc[g] = 0.0f;
+    for (int j = 0; j < QP; j++) acc[j] = 0.0f;
+    const int d = tid % HD, part = tid / HD;
     for (uint32_t c0 = (uint32_t)begin; c0 < stop; c0 += CHUNK) {
-        __syncthreads();
-        const uint32_t pos = c0 + tid;
-        const bool live = pos < stop;
-        float s[G];
-#pragma unroll
-        for (int g = 0; g < G; g++) s[g] = live ? 0.0f : -INFINITY;
-        if (live) {
-            uint32_t id = list[pos / p.capacity];
+        const int live = (int)min(stop - c0, (uint32_t)CHUNK);
+        __syncthreads();  // the chunk before is done with
+        for (int i = tid; i < CHUNK * (HD / 4); i += F32_THREADS) {
+            const int r = i / (HD / 4), x = i % (HD / 4) * 4;
+            const uint32_t pos = c0 + min(r, live - 1);
+            uint32_t id = __ldg(list + pos / p.capacity);
             if (id >= p.slots) {
                 atomicExch(err, ERR_BAD_INDEX);
                 id = 0;
             }
-            from[tid] = (((uint64_t)id * kvh + kv) * p.capacity + pos % p.capacity) * HD;
-            const typename Vec<T>::Raw *kr = reinterpret_cast<const typename Vec<T>::Raw *>(k + from[tid]);
+            const size_t from = (((size_t)id * kvh + kv) * p.capacity + pos % p.capacity) * HD + x;
+            fa::cp_async16(ks + r * C::KROW + x, k + from, r < live);
+            fa::cp_async16(vs + r * HD + x, v + from, r < live);  // zero past the piece: 0 x NaN is NaN
+        }
+        fa::cp_async_commit();
+        fa::cp_async_wait<0>();
+        __syncthreads();
+        {
+            const int key = tid % CHUNK, half = tid / CHUNK;
+            float s[QH];
+#pragma unroll
+            for (int j = 0; j < QH; j++) s[j] = 0.0f;
 #pragma unroll 4
-            for (int d = 0; d < HD / Vec<T>::N; d++) {
-                float f[Vec<T>::N];
-                Vec<T>::unpack(__ldg(kr + d), f);
+            for (int x = 0; x < HD; x += 4) {
+                const float4 kx = *reinterpret_cast<const float4 *>(ks + key * C::KROW + x);
 #pragma unroll
-                for (int g = 0; g < G; g++)
-                    if (g < group)
+                for (int j = 0; j < QH; j++) {
+                    const float4 qx = *reinterpret_cast<const float4 *>(qs + (half * QH + j) * HD + x);
+                    s[j] = __fmaf_rn(kx.w, qx.w, __fmaf_rn(kx.z, qx.z, __fmaf_rn(kx.y, qx.y, __fmaf_rn(kx.x, qx.x, s[j]))));
+                }
+            }
 #pragma unroll
-                        for (int e = 0; e < Vec<T>::N; e++) s[g] = __fmaf_rn(f[e], qs[g][d * Vec<T>::N + e], s[g]);
+            for (int j = 0; j < QH; j++) es[(half * QH + j) * CHUNK + key] = key < live ? s[j] : -INFINITY;
+        }
+        __syncthreads();
+        for (int j = warp; j < queries; j += F32_THREADS / 32) {
+            float e[CHUNK / 32], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < CHUNK / 32; i++) top = fmaxf(top, e[i] = es[j * CHUNK + i * 32 + lane]);
+            const float m0 = mrun[j], l0 = lrun[j], m = fmaxf(m0, warp_max(top));
+#pragma unroll
+            for (int i = 0; i < CHUNK / 32; i++) {
+                const float x = e[i] == -INFINITY ? 0.0f : expf(e[i] - m);
+                es[j * CHUNK + i * 32 + lane] = x;
+                sum += x;
+            }
+            const float l = warp_sum(sum), keep = m0 == -INFINITY ? 0.0f : expf(m0 - m);
+            if (lane == 0) {
+                mrun[j] = m;
+                lrun[j] = __fmaf_rn(l0, keep, l);
+                keep_s[j] = keep;
             }
         }
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-            const float m = warp_max(s[g]);
-            if (lane == 0) red[g][warp] = m;
-        }
-        __syncthreads();
-        if (tid < G) {
-            float m = mrun[tid];
-            for (int w = 0; w < CHUNK / 32; w++) m = fmaxf(m, red[tid][w]);
-            alpha[tid] = mrun[tid] == -INFINITY ? 0.0f : expf(mrun[tid] - m);
-            mrun[tid] = m;
-        }
         __syncthreads();
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-            const float e = s[g] == -INFINITY ? 0.0f : expf(s[g] - mrun[g]);
-            es[g][tid] = e;
-            const float l = warp_sum(e);
-            if (lane == 0) red[g][warp] = l;
-        }
-        __syncthreads();
-        if (tid < G) {
-            float l = lrun[tid] * alpha[tid];
-            for (int w = 0; w < CHUNK / 32; w++) l += red[tid][w];
-            lrun[tid] = l;
-        }
-        const int d = tid % HD, half = tid / HD, count = (int)min((uint32_t)CHUNK, stop - c0);
+        for (int j = 0; j < QP; j++)
+            if (part * QP + j < queries) acc[j] *= keep_s[part * QP + j];
+#pragma unroll 2
+        for (int x = 0; x < CHUNK; x += 4) {
+            const float v0 = vs[x * HD + d], v1 = vs[(x + 1) * HD + d], v2 = vs[(x + 2) * HD + d], v3 = vs[(x + 3) * HD + d];
 #pragma unroll
-        for (int g = 0; g < G; g++) acc[g] *= alpha[g];
-        for (int i = half; i < count; i += HALVES) {
-            const float x = to_f32<T>(v[from[i] + d]);
-#pragma unroll
-            for (int g = 0; g < G; g++) acc[g] = __fmaf_rn(es[g][i], x, acc[g]);
+            for (int j = 0; j < QP; j++) {
+                const float4 e = *reinterpret_cast<const float4 *>(es + (part * QP + j) * CHUNK + x);
+                acc[j] = __fmaf_rn(e.w, v3, __fmaf_rn(e.z, v2, __fmaf_rn(e.y, v1, __fmaf_rn(e.x, v0, acc[j]))));
+            }
         }
     }
-    if (HALVES > 1) {
-        __syncthreads();
-        if (tid >= HD)
+    const uint32_t piece = SHARED ? index : np + index;
 #pragma unroll
-            for (int g = 0; g < G; g++) add[g][tid - HD] = acc[g];
-        __syncthreads();
-        if (tid < HD)
-#pragma unroll
-            for (int g = 0; g < G; g++) acc[g] += add[g][tid];
+    for (int j = 0; j < QP; j++) {
+        const int x = part * QP + j;
+        if (x < queries) out.o[(head_of(x) * pieces + piece) * HD + d] = acc[j];
     }
-    __syncthreads();
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        if (g >= group) break;
-        const size_t to = ((size_t)row * heads + kv * group + g) * pieces + piece;
-        if (tid < HD) out.o[to * HD + tid] = acc[g];
-        if (tid == 0) *reinterpret_cast<float2 *>(out.ml + to * 2) = make_float2(mrun[g], lrun[g]);
+    if (tid < queries) *reinterpret_cast<float2 *>(out.ml + (head_of(tid) * pieces + piece) * 2) = make_float2(mrun[tid], lrun[tid]);
+}
+
+// Blocks of the shared pieces first (they take longer), then those of the rows' own; a block to a KV head in y.
+template <int HD>
+__global__ void __launch_bounds__(F32_THREADS)
+    f32_kernel(tg_params p, const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
+               const uint32_t *__restrict__ at, const uint32_t *__restrict__ table, const uint32_t *__restrict__ shared, Partials out,
+               uint32_t np, uint32_t pieces, uint32_t far, uint32_t *err) {
+    pdl_wait();
+    pdl_launch_dependents();
+    if (blockIdx.x < far)
+        f32_piece<HD, F32_QUERIES, true>(p, q, k, v, at, table, shared, out, blockIdx.x % np, blockIdx.y, blockIdx.x / np, np, pieces, err);
+    else {
+        const uint32_t b = blockIdx.x - far, own = pieces - np;
+        f32_piece<HD, MAX_GROUP, false>(p, q, k, v, at, table, shared, out, b % own, blockIdx.y, b / own, np, pieces, err);
     }
 }
 
@@ -904,9 +933,15 @@ cudaError_t attend(const tg_params &p, const void *q_, const void *k_, const voi
         return launch_pdl(join_kernel<T, HD>, dim3((unsigned)items), dim3(JOIN_THREADS), 0, s, p, at, part, np, pieces, out);
     };
     if constexpr (sizeof(T) == 4) {
+        auto kernel = f32_kernel<HD>;
+        constexpr int SMEM = F32<HD, F32_QUERIES>::SMEM;
+        const cudaError_t e = with_all_smem(kernel, SMEM);
+        if (e != cudaSuccess) return e;
+        const uint32_t tile_rows = F32_QUERIES / (p.heads / p.kv_heads), far = np * ((p.rows + tile_rows - 1) / tile_rows);
+        const uint64_t blocks = far + (uint64_t)p.rows * (pieces - np);
         run = [=](cudaStream_t s) {
-            const cudaError_t e = launch_pdl(pieces_kernel<T, HD>, dim3(pieces, p.kv_heads, p.rows), dim3(CHUNK), 0, s, p, q, k, v, at, table,
-                                             shared, part, np, pieces, err);
+            const cudaError_t e = launch_pdl(kernel, dim3((unsigned)blocks, p.kv_heads), dim3(F32_THREADS), SMEM, s, p, q, k, v, at, table,
+                                             shared, part, np, pieces, far, err);
             return e != cudaSuccess ? e : join(s);
         };
     } else {
