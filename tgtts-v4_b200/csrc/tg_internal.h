@@ -243,7 +243,7 @@ cudaError_t launch_gemm_silu(const tg_params &p, const void *a, const void *b, v
 
 // A paged, prefix-sharing batch (kernels_paged.cu, attention_pages.cu).
 constexpr uint32_t PAGE_STEP = 16;           // a page's positions are a multiple of this
-constexpr uint32_t PLAN_MAX_SEQS = 16384;    // page_plan's requests: its two sums of each in shared memory
+constexpr uint32_t PLAN_MAX_SEQS = 16384;    // page_plan's requests: three words of each in shared memory
 cudaError_t launch_page_plan(const tg_params &p, const uint32_t *held, const uint32_t *fresh, const uint32_t *free,
                              uint32_t *table, uint32_t *at, uint32_t *place, uint32_t *starts, uint32_t *next,
                              uint32_t *counts, uint32_t *err, cudaStream_t s);
