@@ -22,14 +22,20 @@ constexpr uint32_t SPARE = TG_SPARE;
 
 // Own positions of a piece.
 constexpr uint32_t OWN_PIECE = 128;
-// Shared positions of a piece: at most 16 pieces, each whole tiles of 128.
-__host__ __device__ inline uint32_t shared_piece(uint32_t first) {
-    const uint32_t even = (first + 15) / 16;
-    return even <= 128 ? 128 : (even + 127) / 128 * 128;
+// n / d, rounded up.
+__host__ __device__ inline uint32_t shares(uint32_t n, uint32_t d) { return n / d + (n % d != 0); }
+// Shared positions of a piece, whole tiles of 128: at most 16 pieces; 8 while those are at most 512 and at most 64 x KV
+// heads long, as the KV heads make units too. (Behind 4096 positions, 8 KV heads of 128, pieces of 512 against 256: 32 rows
+// 19.6 us against 24.7, 128 rows 75 against 84, one row 13.7 against 12.1. Behind 16384 pieces of 2048 against 1024: 64 rows
+// 53 against 55, one row 29 against 20.)
+__host__ __device__ inline uint32_t shared_piece(const tg_params &p) {
+    const uint32_t most = p.kv_heads < 8 ? 64 * p.kv_heads : 512, even = shares(p.first, 8);
+    const uint32_t longer = even < most ? even : most, size = longer > shares(p.first, 16) ? longer : shares(p.first, 16);
+    return size ? shares(size, 128) * 128 : 128;
 }
-__host__ __device__ inline uint32_t shared_pieces(uint32_t first) { return (first + shared_piece(first) - 1) / shared_piece(first); }
+__host__ __device__ inline uint32_t shared_pieces(const tg_params &p) { return shares(p.first, shared_piece(p)); }
 __host__ __device__ inline uint64_t all_pieces(const tg_params &p) {
-    return shared_pieces(p.first) + ((uint64_t)p.stride * p.capacity + OWN_PIECE - 1) / OWN_PIECE;
+    return shared_pieces(p) + ((uint64_t)p.stride * p.capacity + OWN_PIECE - 1) / OWN_PIECE;
 }
 
 // The partials in the work buffer, from its first 256-byte boundary: o f32 [rows][heads][pieces][hd], then
@@ -83,7 +89,7 @@ __device__ __forceinline__ void f32_piece(const tg_params &p, const float *__res
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, heads = p.heads, kvh = p.kv_heads, group = heads / kvh;
     const int rows = SHARED ? QN / group : 1, row0 = tile * rows, queries = min(rows, (int)p.rows - row0) * group;
     uint32_t length = p.first, seq = 0;
-    const uint32_t size = SHARED ? shared_piece(p.first) : OWN_PIECE;
+    const uint32_t size = SHARED ? shared_piece(p) : OWN_PIECE;
     const uint64_t begin = (uint64_t)index * size;
     if ((!SHARED && !paged_row(p, at, row0, length, seq, kv == 0 && index == 0 && tid == 0 ? err : nullptr)) || begin >= length) return;
     const uint32_t stop = (uint32_t)min((uint64_t)length, begin + size);
@@ -497,7 +503,7 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS) __maxnreg__(Pfx<HD>::REGS)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     const int heads = p.heads, kvh = p.kv_heads, group = heads / kvh, tile_rows = 128 / group;
     const int tiles = ((int)p.rows + tile_rows - 1) / tile_rows, pairs = (tiles + C::NT - 1) / C::NT;
-    const uint32_t size = shared_piece(p.first), np = shared_pieces(p.first), units = np * pairs * kvh;
+    const uint32_t size = shared_piece(p), np = shared_pieces(p), units = np * pairs * kvh;
     auto B = [](uint64_t &b) { return smem_u32(&b); };
 
     if (tid == 0) {
@@ -928,7 +934,7 @@ cudaError_t attend(const tg_params &p, const void *q_, const void *k_, const voi
     T *out = static_cast<T *>(out_);
     float *o = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(work) + 255) & ~uintptr_t(255));
     const Partials part{o, o + items * all * HD};
-    const uint32_t np = shared_pieces(p.first), pieces = (uint32_t)all;
+    const uint32_t np = shared_pieces(p), pieces = (uint32_t)all;
     auto join = [=](cudaStream_t s) {
         return launch_pdl(join_kernel<T, HD>, dim3((unsigned)items), dim3(JOIN_THREADS), 0, s, p, at, part, np, pieces, out);
     };
