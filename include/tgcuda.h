@@ -265,7 +265,7 @@ typedef enum {
      * largest stored value above -inf (never a NaN), TG_SPARE when there is none. Tokens past the
      * vocabulary in seen or bias_ids count for nothing. A span past its array, or a mask of m or
      * more, leaves the row's out and pick as they were, with the kernel error word. k, k1 and m may
-     * be 0 (the arrays then any 16 bytes). A row's generated tokens: at most 2^30 - 1. */
+     * be 0 (the arrays then any 16 bytes). k is below 2^30 (a token's count is held in 30 bits). */
     TG_KERNEL_LOGITS_PICK = 30,
     TG_KERNEL_COUNT = 31
 } tg_kernel_id;

@@ -78,7 +78,8 @@ def test_logits_pick_bindings(pkg):
     assert pkg.needs("logits_pick", pick(pkg, dtype=1, k=0, k1=0, m=0)) == [6048, 16, 72, 36, 16, 16, 16, 6048, 12]
 
 
-@pytest.mark.parametrize("kw", [dict(n=0), dict(stride=999), dict(rows=0), dict(rows=65536), dict(dtype=2), dict(n=1 << 31, stride=1 << 31)])
+@pytest.mark.parametrize("kw", [dict(n=0), dict(stride=999), dict(rows=0), dict(rows=65536), dict(dtype=2), dict(n=1 << 31, stride=1 << 31),
+                                dict(k=1 << 30)])
 def test_logits_pick_refuses(pkg, kw):
     with pytest.raises(pkg.ShapeError):
         pkg.needs("logits_pick", pick(pkg, **kw))

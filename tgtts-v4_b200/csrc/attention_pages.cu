@@ -72,7 +72,7 @@ template <int HD, int QN>
 struct F32 {
     static constexpr int CHUNK = 8192 / HD;  // keys at once
     static constexpr int KROW = HD + 4;  // floats of a key: eight keys' same 16 bytes lie in all banks
-    static constexpr int V = CHUNK * KROW, Q = V + CHUNK * HD, E = Q + QN * HD, SMEM = (E + QN * CHUNK) * 4;
+    static constexpr int V = CHUNK * KROW, Q = V + CHUNK * HD, E = Q + QN * HD, FLOATS = E + QN * CHUNK;
 };
 
 template <int HD, int QN, bool SHARED>
@@ -940,7 +940,8 @@ cudaError_t attend(const tg_params &p, const void *q_, const void *k_, const voi
     };
     if constexpr (sizeof(T) == 4) {
         auto kernel = f32_kernel<HD>;
-        constexpr int SMEM = F32<HD, F32_QUERIES>::SMEM;
+        constexpr int SMEM = F32<HD, F32_QUERIES>::FLOATS * sizeof(float);
+        static_assert(SMEM >= F32<HD, MAX_GROUP>::FLOATS * sizeof(float), "the own pieces' too");
         const cudaError_t e = with_all_smem(kernel, SMEM);
         if (e != cudaSuccess) return e;
         const uint32_t tile_rows = F32_QUERIES / (p.heads / p.kv_heads), far = np * ((p.rows + tile_rows - 1) / tile_rows);

@@ -275,9 +275,9 @@ static int check_paged_shape(const Launch &l) {
     const char *name = kernel_name(l.kernel);
     if (p.rows == 0) return fail(TG_ESHAPE, "%s: 0 rows", name);
     if (l.kernel == TG_KERNEL_LOGITS_PICK) {
-        if (p.n == 0 || p.n > 0x7fffffffu || p.stride < p.n || p.rows > 65535)
-            return fail(TG_ESHAPE, "logits_pick: %u tokens in rows of %u, %u rows (1 to 2^31 - 1 tokens, at most 65535 rows)",
-                        p.n, p.stride, p.rows);
+        if (p.n == 0 || p.n > 0x7fffffffu || p.stride < p.n || p.rows > 65535 || p.k >= 1u << 30)
+            return fail(TG_ESHAPE, "logits_pick: %u tokens in rows of %u, %u rows, %u seen (1 to 2^31 - 1 tokens, at most 65535 rows, fewer than 2^30 seen)",
+                        p.n, p.stride, p.rows, p.k);
         return TG_OK;
     }
     if (p.capacity == 0 || p.capacity % PAGE_STEP || p.slots == 0 || (uint64_t)p.capacity * p.slots >= TG_SPARE)
