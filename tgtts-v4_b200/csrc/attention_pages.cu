@@ -45,10 +45,8 @@ struct Partials {
 };
 constexpr uint32_t OWN_ROWS = 512;  // rows whose own pieces are listed at once
 
-// A row's own length and request; false for a row that computes nothing.
-TG_DEVICE bool paged_row(const tg_params &p, const uint32_t *at, int row, uint32_t &length, uint32_t &seq, uint32_t *err) {
-    const uint32_t pos = at[row];
-    seq = at[p.rows + row];
+// A row's own length, of its position and request; false for a row that computes nothing.
+TG_DEVICE bool paged_words(const tg_params &p, uint32_t pos, uint32_t seq, uint32_t &length, uint32_t *err) {
     if (pos == SPARE) return false;
     length = pos - p.first + 1;
     if (pos < p.first || (uint64_t)length > (uint64_t)p.stride * p.capacity || seq >= p.seqs) {
@@ -56,6 +54,11 @@ TG_DEVICE bool paged_row(const tg_params &p, const uint32_t *at, int row, uint32
         return false;
     }
     return true;
+}
+TG_DEVICE bool paged_row(const tg_params &p, const uint32_t *at, int row, uint32_t &length, uint32_t &seq, uint32_t *err) {
+    const uint32_t pos = at[row];
+    seq = at[p.rows + row];
+    return paged_words(p, pos, seq, length, err);
 }
 
 // ---- f32, on the CUDA cores ----------------------------------------------------------------------------
@@ -227,7 +230,13 @@ TG_DEVICE uint64_t mn_desc(uint32_t addr, uint32_t chunk) {
 // A warp to a piece of a row's own positions for one KV head, in chunks of own_chunk positions: the group's
 // query heads, at most 8, are the columns of mma.sync.m16n8k16 (S^T = K q^T, O^T = V^T e^T with e split
 // into bf16 hi + lo, against a reference that moves as prefix_kernel's), keys and values gathered from their
-// pages by cp.async, OWN_STAGES - 1 chunks ahead of the products.
+// pages by cp.async, OWN_STAGES - 1 chunks ahead of the products. e keeps 16 bits because a row's own positions are
+// few and may carry its whole sum; the second product costs nothing here, as the caches' bytes bound the
+// kernel: a head reads 4 hd bytes a position for 4 hd x group operations. What is needed is bytes in flight: 11
+// one-warp blocks an SM of two 8 KB stages each hold 90 KB of them, and, as small blocks, find room beside
+// prefix_kernel's (four warps to a block: 64 rows of 1024 behind 16384 positions 67 us against 55). 64 rows of up to 1024, 8 KV
+// heads of 128 (142 MB): 34 us with the join, 4.2 TB/s; 128 rows (268 MB) 56 us, 4.8 TB/s. Pieces of 128
+// positions, so that the longest row is no one warp's.
 constexpr int OWN_WARPS = 1, OWN_STAGES = 2;
 constexpr int own_chunk(int hd) { return 2048 / hd; }
 constexpr int OWN_STAGE = 2 * 2048;  // bf16 of a chunk's keys and values
@@ -269,44 +278,72 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
         __syncthreads();  // the rows before are done with their list
         if (warp == 0) {
             uint32_t total = 0;
-            for (uint32_t r0 = 0; r0 < rows; r0 += 32) {
-                uint32_t length, seq, n = 0;
-                if (r0 + lane < rows && paged_row(p, at, row0 + r0 + lane, length, seq, blockIdx.x == 0 ? err : nullptr))
-                    n = (length + OWN_PIECE - 1) / OWN_PIECE;
-                uint32_t upto = n;
+            constexpr int AT_ONCE = 4;  // loads of 32 rows' words in flight
+            for (uint32_t r0 = 0; r0 < rows; r0 += 32 * AT_ONCE) {
+                uint32_t pos[AT_ONCE], seq[AT_ONCE];
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += u;
+                for (int i = 0; i < AT_ONCE; i++) {
+                    const uint32_t r = r0 + 32 * i + lane;
+                    pos[i] = r < rows ? at[row0 + r] : SPARE;
+                    seq[i] = r < rows ? at[p.rows + row0 + r] : 0;
                 }
-                if (r0 + lane < rows) first_piece[r0 + lane] = total + upto - n;
-                total += __shfl_sync(0xffffffffu, upto, 31);
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; i++) {
+                    const uint32_t r = r0 + 32 * i + lane;
+                    uint32_t length, n = 0;
+                    if (paged_words(p, pos[i], seq[i], length, blockIdx.x == 0 ? err : nullptr)) n = (length + OWN_PIECE - 1) / OWN_PIECE;
+                    uint32_t upto = n;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += u;
+                    }
+                    if (r < rows) first_piece[r] = total + upto - n;
+                    total += __shfl_sync(0xffffffffu, upto, 31);
+                }
             }
             if (lane == 0) total_s = total;
         }
         __syncthreads();
-        const uint64_t tasks = (uint64_t)total_s * kvh;
-        for (uint64_t task = (uint64_t)blockIdx.x * OWN_WARPS + warp; task < tasks; task += (uint64_t)gridDim.x * OWN_WARPS) {
-            const uint32_t u = (uint32_t)(task / kvh);
-            const int kv = (int)(task % kvh);
+        // (Fewer than 2^32: each has partials of 264 bytes or more in the work buffer.)
+        const uint32_t tasks = total_s * kvh, step = gridDim.x * OWN_WARPS;
+        // A task, and the words that lead to its pages: they are on their way while the one before is computed.
+        uint32_t row_n, piece_n, pos_n, seq_n, id_n = 0;
+        auto find = [&](uint32_t task) {
+            if (task >= tasks) return;
+            const uint32_t u = task / kvh;
             uint32_t lo = 0, hi = rows;  // the row with first_piece at most u, its next above
             while (hi - lo > 1) {
                 const uint32_t mid = (lo + hi) / 2;
                 if (first_piece[mid] <= u) lo = mid;
                 else hi = mid;
             }
-            const uint32_t row = row0 + lo, piece = u - first_piece[lo], begin = piece * OWN_PIECE;
-            const int live = (int)min(at[row] - p.first + 1 - begin, OWN_PIECE), chunks = (live + CH - 1) / CH;
-            // Where positions begin + 16 i .. lie in the caches (16 share a page): lane i < 8.
+            row_n = row0 + lo;
+            piece_n = u - first_piece[lo];
+            pos_n = at[row_n];
+            seq_n = at[p.rows + row_n];
+        };
+        auto live_of = [&](uint32_t pos, uint32_t piece) { return (int)min(pos - p.first + 1 - piece * OWN_PIECE, OWN_PIECE); };
+        // Positions piece x OWN_PIECE + 16 i .. share a page: lane i < 8.
+        auto place_of = [&](uint32_t piece, int live) { return piece * OWN_PIECE + min(16 * (lane & 7), (live - 1) & ~15); };
+        auto fetch = [&](uint32_t task) {
+            if (task < tasks) id_n = __ldg(table + (size_t)seq_n * p.stride + place_of(piece_n, live_of(pos_n, piece_n)) / p.capacity);
+        };
+        const uint32_t task0 = blockIdx.x * OWN_WARPS + warp;
+        find(task0);
+        fetch(task0);
+        for (uint32_t task = task0; task < tasks; task += step) {
+            const int kv = (int)(task % kvh);
+            const uint32_t row = row_n, piece = piece_n;
+            const int live = live_of(pos_n, piece_n), chunks = (live + CH - 1) / CH;
             uint64_t from;
             {
-                const uint32_t pos = begin + min(16 * (lane & 7), (live - 1) & ~15);
-                uint32_t id = __ldg(table + (size_t)at[p.rows + row] * p.stride + pos / p.capacity);
+                uint32_t id = id_n;
                 if (id >= p.slots) {
                     atomicExch(err, ERR_BAD_INDEX);
                     id = 0;
                 }
-                from = (((uint64_t)id * kvh + kv) * p.capacity + pos % p.capacity) * HD;
+                from = (((uint64_t)id * kvh + kv) * p.capacity + place_of(piece, live) % p.capacity) * HD;
             }
             const int in_row = lane % VECS, in_group = lane / VECS;
             auto gather = [&](int c) {
@@ -329,6 +366,7 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
                 if (c < chunks) gather(c);
                 cp_async_commit();
             }
+            find(task + step);
             // q of the group's heads as columns g < group of the products (those past it zero).
             uint32_t qf[HD / 16][2];
             const bf16 *qg = q + ((size_t)row * heads + kv * group + g) * HD + 2 * t4;
@@ -346,6 +384,7 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
                 __syncwarp();  // the chunk is in, and every lane is done with the one before
                 if (c + OWN_STAGES - 1 < chunks) gather(c + OWN_STAGES - 1);
                 cp_async_commit();
+                if (c == 0) fetch(task + step);
                 const bf16 *ks = stages + (c % OWN_STAGES) * OWN_STAGE, *vs = ks + CH * HD;
                 float sc[G16][4];  // positions g and g + 8 of each 16, the lane's two heads
                 const int left = live - c * CH - g;
@@ -436,7 +475,8 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
 
 // ---- shared pieces, bf16 ------------------------------------------------------------------------------
 // A block an SM, over units of a piece, a KV head and NT tiles of up to 128 queries, query m of a tile being
-// head m % group of row m / group of the tile's rows, against the piece's keys in tiles of 128. Twelve warps (eight for one tile; warp 3 has no part):
+// head m % group of row m / group of the tile's rows, against the piece's
+// keys in tiles of 128. Twelve warps (eight for one tile; warp 3 has no part):
 //   warps 0 and 2  TMA: Q and the K tiles, and the V tiles, page by page (boxes of the largest of
 //              128, 64, 32 and 16 positions that divides a page) into STAGES stages of
 //              128-byte-swizzled halves of 64 dimensions; values past the prefix in its last tile set to
@@ -446,10 +486,17 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
 //              read MN-major), the tile's next S ahead of its PV so that the softmax runs under it;
 //   warps 4-7  (and 8-11)  the softmax of a tile, a thread to a query: P_j = 2^(S_j scale - mref) as bf16
 //              into TMEM against a reference that moves only when a tile's maximum passes it by 2^8 (O
-//              then rescaled in place), the same pass as the prefill's attention kernel.
+//              then rescaled in place), the same pass as the prefill's attention kernel. P is rounded to
+//              bf16 for the product (by 2^-8 of its value at most; the errors of many keys average out);
+//              its sum l is of the f32 values.
 // HD = 64: two tiles, which share the keys' copies, each with S, P and O in 256 columns. HD = 128: one tile
 // with two S buffers (S 2 x 128, P 64, O 128), as two tiles do not fit TMEM's 512 columns.
 // The softmax warps take registers from the first four (setmaxnreg), so that own_kernel's blocks find room beside.
+// A tile of 128 keys takes about 2400 clocks (hd 64: 3400 for two tiles of queries), of which a softmax thread's
+// exponentials and sums are 1400, its waits and TMEM's loads and stores the rest; keys and values come
+// from L2 at up to 7.5 TB/s over all SMs meanwhile. No part bounds it alone: without the exponentials, or most of the
+// products, or with P in two places, the time is the same within 3%. Storing a unit's partials takes 5000 clocks.
+// Alone: 128 rows of 16 heads over 2 of 64 behind 8191 positions 15.5 us, 64 rows of 32 over 8 of 128 behind 16384 33 us.
 // Every wait is bounded (the context's error word, then the block runs out).
 template <int HD>
 struct Pfx {
@@ -723,8 +770,9 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS) __maxnreg__(Pfx<HD>::REGS)
                     mbar_wait(B(bs_full[h * C::SB + (C::SB - 1) * (t & 1)]), (t / C::SB) & 1, err, &gave_up);
                     tc_fence_after();
                     // P_j against mref into TMEM with its sum, the tile's raw maximum alongside; P_j takes P_{j-1}'s place once
-                    // PV_{j-1} has read it. (The first tile's first half of keys gives the first reference.) Where the maximum has passed a reference by MOVE_PAST, O (with PV_{j-1} in it) is
-                    // rescaled, a query that keeps its reference times 1, and the warp's pass runs again from S_j.
+                    // PV_{j-1} has read it. (The first tile's first half of keys gives the first reference.) Where the maximum
+                    // has passed a reference by MOVE_PAST, O (with PV_{j-1} in it) is rescaled, a query that keeps its
+                    // reference times 1, and the warp's pass runs again from S_j.
                     float a = 1.0f, sum;
                     for (bool again = false;; again = true) {
                         float2 sums[4];
@@ -834,7 +882,8 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS) __maxnreg__(Pfx<HD>::REGS)
 
 // Joins the partials of a row's head, a block to it: 16 bytes of a piece's o to a lane, the pieces over the
 // block's groups of HD / 4 lanes, all loads of a row of up to JOIN_DEEP pieces a group in flight at once; the
-// groups' sums are then added in order. References are in base 2 for bf16, natural for f32.
+// groups' sums are then added in order. References are in base 2 for bf16, natural for f32. Latency-bound, then by
+// the partials' bytes from L2: 2048 heads of 16 + 2 pieces of 64 5 us, of 16 + 5 pieces of 128 9 us.
 constexpr int JOIN_THREADS = 128, JOIN_DEEP = 8;
 
 template <typename T, int HD>
