@@ -322,7 +322,7 @@ constexpr int PICK_THREADS = 512;
 constexpr uint32_t PICK_TILE = 1024, PICK_AHEAD = 64 * PICK_TILE;
 constexpr uint32_t PICK_RUN = 65536;     // the most tokens whose bits are held at once
 constexpr uint32_t PICK_TOUCHED = 4096;  // the most touched tokens whose words are held at once
-constexpr size_t PICK_SMEM = (PICK_RUN / 32 + 3 * PICK_TOUCHED) * sizeof(uint32_t) + PICK_RUN / 32 * sizeof(uint16_t);
+constexpr size_t PICK_SMEM = (PICK_RUN / 32 + 2 * PICK_TOUCHED) * sizeof(uint32_t) + (PICK_TOUCHED + PICK_RUN / 32) * sizeof(uint16_t);
 // A count word: the prompt holds the token; a bias names it; below, its generated occurrences.
 constexpr uint32_t IN_PROMPT = 1u << 31, BIASED = 1u << 30;
 
@@ -347,10 +347,10 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
     constexpr uint32_t STEP = PICK_THREADS * VEC * EACH, ALL = (1u << VEC) - 1;
     extern __shared__ __align__(16) uint32_t pick_smem[];
     uint32_t *touched = pick_smem, *count = touched + PICK_RUN / 32, *biased = count + PICK_TOUCHED;
-    ushort2 *token = reinterpret_cast<ushort2 *>(biased + PICK_TOUCHED);  // touched tokens, and where they are counted
+    uint16_t *token = reinterpret_cast<uint16_t *>(biased + PICK_TOUCHED);  // the touched tokens in order
     uint16_t *before = reinterpret_cast<uint16_t *>(token + PICK_TOUCHED);
     __shared__ Best warp_best[PICK_THREADS / 32], block_best[8];  // the first block's: of every block
-    __shared__ uint32_t warp_bits[PICK_THREADS / 32], listed;
+    __shared__ uint32_t warp_bits[PICK_THREADS / 32];
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t row = blockIdx.x / ranks, n = p.n;
@@ -389,6 +389,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
                 if (t + VEC <= n) raw[j] = __ldcs(reinterpret_cast<const Raw *>(x + t));
             }
         };
+        uint32_t total = 0;  // touched tokens
         if (!controls) load(l0);
         auto allow = [&](uint32_t t) { return bits ? __ldg(bits + t / 32) >> (t % 32) : 0xffffffffu; };
         auto hits = [&](uint32_t in) { return controls ? touched[in / 32] >> (in % 32) & ALL : 0u; };
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
             };
             constexpr uint32_t LINE = 128 / sizeof(T);
             constexpr uint32_t W = PICK_RUN / 32 / PICK_THREADS;  // words of the bit map to a thread
-            uint32_t total, upto, marks[W];
+            uint32_t upto, marks[W];
             while (true) {
                 __syncthreads();  // the run before is done with the words
 #pragma unroll
@@ -456,14 +457,14 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
                 upto += __popc(marks[i]);
             }
             for (uint32_t i = tid; i < total; i += PICK_THREADS) count[i] = biased[i] = 0;
-            if (tid == 0) listed = 0;
             __syncthreads();
-            // The entry that finds its token's count zero lists the token.
+            // (The entries of a token all write the same number of it.)
             auto add = [&](uint32_t in, uint32_t i, uint32_t first) {
                 const uint32_t at = before[in / 32] + __popc(touched[in / 32] & ((1u << (in % 32)) - 1));
-                const uint32_t old = first == 1 ? atomicAdd(count + at, 1u) : atomicOr(count + at, first);
+                if (first == 1) atomicAdd(count + at, 1u);
+                else atomicOr(count + at, first);
                 if (first == BIASED) atomicMax(biased + at, i + 1);
-                if (old == 0) token[atomicAdd(&listed, 1u)] = make_ushort2(in, at);
+                token[at] = (uint16_t)in;
             };
             entries([&](uint32_t in, uint32_t i) { add(in, i, i < prompt ? IN_PROMPT : 1u); }, [&](uint32_t in, uint32_t i) { add(in, i, BIASED); });
             __syncthreads();
@@ -475,7 +476,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
                 for (int k = 0; k < F; k++) {
                     const uint32_t i = i0 + k * PICK_THREADS;
                     if (i >= total) continue;
-                    const uint32_t t = token_of(l0 + token[i].x);
+                    const uint32_t t = token_of(l0 + token[i]);
                     value[k] = x[t];
                     all[k] = allow(t);
                 }
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
                 for (int k = 0; k < F; k++) {
                     const uint32_t i = i0 + k * PICK_THREADS;
                     if (i >= total) continue;
-                    const uint32_t t = token_of(l0 + token[i].x), c = count[token[i].y], b = biased[token[i].y], made = c & (BIASED - 1);
+                    const uint32_t t = token_of(l0 + token[i]), c = count[i], b = biased[i], made = c & (BIASED - 1);
                     float f = to_f32<T>(value[k]);
                     if (c & ~BIASED) {
                         f = f > 0.0f ? __fdiv_rn(f, repetition) : f * repetition;
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
                     }
                     if (b) f = f + bias[bias0 + b - 1];
                     const float stored = to_f32<T>(from_f32<T>(all[k] & 1 ? f : -INFINITY));
-                    biased[token[i].y] = __float_as_uint(stored);  // stored behind the stream
+                    biased[i] = __float_as_uint(stored);  // stored behind the stream
                     if (stored > -INFINITY) better(other, stored, t);
                 }
             }
@@ -531,7 +532,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
         }
         if (controls) {
             __syncthreads();  // the touched tokens' logits over what the stream left there
-            for (uint32_t i = tid; i < listed; i += PICK_THREADS) y[token_of(l0 + token[i].x)] = from_f32<T>(__uint_as_float(biased[token[i].y]));
+            for (uint32_t i = tid; i < total; i += PICK_THREADS) y[token_of(l0 + token[i])] = from_f32<T>(__uint_as_float(biased[i]));
         }
     }
     better(best, other.value, other.token);
