@@ -212,7 +212,8 @@ TG_DEVICE bool rope_row(const tg_params &p, uint32_t pos, uint32_t to, uint32_t 
 // For a rotated part that is a multiple of 8: a thread takes eight dimensions of two heads (h and h + half the heads,
 // which turn by the same angles), rotated ones as four pairs (in the half layout two runs of four, each a warp's
 // whole sectors), of every gridDim-th group of rows: where they lie in a row is worked out once. All of a
-// row's loads of c leave before it is known whether the row is spare.
+// row's loads of c leave before it is known whether the row is spare. 32768 rows of 20 heads of 64, f32 to bf16 (253
+// MB): 45.7 us, 5.5 TB/s; 2047 rows of 48 heads of 128 (50 MB): 10.3 us.
 constexpr int ROPE_THREADS = 256;
 
 template <typename T, typename C, bool INTER, int HD>
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(ROPE_THREADS)
     }
 }
 
-// Any even rotated part: a pair to a thread.
+// Any other even rotated part: a pair to a thread (2047 rows of 48 heads of 128: 31 us, 9 where a thread takes eight).
 template <typename T, typename C>
 __global__ void __launch_bounds__(ROPE_THREADS)
     rope_pages_any_kernel(tg_params p, Divisor page, Divisor row_units, uint32_t block_rows, const uint32_t *__restrict__ at,
@@ -315,9 +316,12 @@ __global__ void __launch_bounds__(ROPE_THREADS)
 // the history or the biases) in a bit map and numbers them by its running bit counts; their occurrences are
 // added, and a token's last bias entry found, atomically on whole numbers, so that no order shows. The
 // touched logits are then done a thread to a token, and the others pass through without a barrier, four
-// or eight to a 16-byte load and store, the first of them on their way since before the counting. The
-// row's greedy choice is joined over the cluster in distributed shared memory. HBM-bound: each logit is
-// read and written once.
+// or eight to a 16-byte load and store (one by one in rows that 16 bytes do not divide); the touched ones' values
+// overwrite what the stream left. The row's greedy choice is joined over the cluster in distributed shared memory.
+// HBM-bound where there are rows enough: each logit is read and written once. 128 rows of 128,000 tokens in f32
+// (131 MB): 24.2 us without controls, 5.4 TB/s; 33 us with histories of 4096 tokens and 64 biases, whose two passes
+// come before the stream (under them the logits come into L2). One row of 32,000 with a history of 700: 6.8 us, the
+// passes' latencies. Counting inside the stream, a table of counts to a tile: 71 us for the 128 rows.
 constexpr int PICK_THREADS = 512;
 constexpr uint32_t PICK_TILE = 1024, PICK_AHEAD = 64 * PICK_TILE;
 constexpr uint32_t PICK_RUN = 65536;     // the most tokens whose bits are held at once
@@ -379,6 +383,11 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
         const uint32_t tile = t / PICK_TILE;
         return t < n && (tile & (ranks - 1)) == rank ? (tile >> rank_bits) * PICK_TILE + t % PICK_TILE : SPARE;
     };
+    constexpr int H = 8;  // entries of a thread in flight
+    auto history_at = [&](uint32_t i0, uint32_t(&e)[H]) {
+#pragma unroll
+        for (int h = 0; h < H; h++) e[h] = i0 + h * PICK_THREADS < history ? __ldg(seen + begin + i0 + h * PICK_THREADS) : SPARE;
+    };
     for (uint32_t l0 = 0, end; l0 < mine; l0 = end) {
         end = min(mine, l0 + PICK_RUN);
         Raw raw[EACH];
@@ -390,24 +399,29 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
             }
         };
         uint32_t total = 0;  // touched tokens
-        if (!controls) load(l0);
         auto allow = [&](uint32_t t) { return bits ? __ldg(bits + t / 32) >> (t % 32) : 0xffffffffu; };
         auto hits = [&](uint32_t in) { return controls ? touched[in / 32] >> (in % 32) & ALL : 0u; };
         if (controls) {
+            // A thread's first entries stay with it for both passes; a token past the vocabulary where there is none.
+            uint32_t first_entries[H];
+            history_at(tid, first_entries);
+            const uint32_t first_bias = tid < biases ? __ldg(bias_ids + bias0 + tid) : SPARE;
             auto entries = [&](auto in_history, auto in_biases) {
-                constexpr int H = 8;  // entries of a thread in flight
-                for (uint32_t i0 = tid; i0 < history; i0 += PICK_THREADS * H) {
-                    uint32_t e[H];
-#pragma unroll
-                    for (int h = 0; h < H; h++) e[h] = i0 + h * PICK_THREADS < history ? __ldg(seen + begin + i0 + h * PICK_THREADS) : SPARE;
+                auto all = [&](const uint32_t(&e)[H], uint32_t i0) {
 #pragma unroll
                     for (int h = 0; h < H; h++) {
                         const uint32_t in = local_of(e[h]) - l0;
                         if (in < end - l0) in_history(in, i0 + h * PICK_THREADS);
                     }
+                };
+                all(first_entries, tid);
+                for (uint32_t i0 = tid + PICK_THREADS * H; i0 < history; i0 += PICK_THREADS * H) {
+                    uint32_t e[H];
+                    history_at(i0, e);
+                    all(e, i0);
                 }
                 for (uint32_t i = tid; i < biases; i += PICK_THREADS) {
-                    const uint32_t in = local_of(bias_ids[bias0 + i]) - l0;
+                    const uint32_t in = local_of(i == tid ? first_bias : bias_ids[bias0 + i]) - l0;
                     if (in < end - l0) in_biases(in, i);
                 }
             };
@@ -501,7 +515,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 2)
         // The stream: logits masked, stored and, untouched ones, compared with the best so far. A thread meets its
         // tokens in ascending order, so that the first of equal values stays.
         for (uint32_t at = l0; at < end; at += STEP) {
-            if (at != l0 || controls) load(at);
+            load(at);
 #pragma unroll
             for (int j = 0; j < EACH; j++) {
                 const uint32_t l = at + (j * PICK_THREADS + tid) * VEC, t = token_of(l);
@@ -560,7 +574,9 @@ template <typename T, int VEC>
 cudaError_t pick_t(const tg_params &p, const void *logits, const uint32_t *seen, const uint32_t *spans, const float *pen,
                    const uint32_t *ids, const float *bias, const uint32_t *masks, void *out, uint32_t *pick, uint32_t *err,
                    cudaStream_t s) {
-    // Blocks of 1024 tokens at least; eight to a row, or four where rows alone fill the device's four blocks an SM.
+    // Blocks of 1024 tokens at least; the most to a row that run at once (two an SM), up to eight. Of 128,000 tokens
+    // with 8, 4 and 2 blocks a row: 1 row 9.1, 12.2, 18.1 us; 32 rows 14.5, 18.3, 24.0; 64 rows 27.5, 20.7, 30.5; 128
+    // rows 54, 39, 34.
     uint32_t ranks = p.rows <= 32 ? 8 : p.rows <= 64 ? 4 : 2;
     while (ranks > 1 && p.n <= ranks / 2 * PICK_TILE) ranks /= 2;
     cudaError_t e = with_smem(logits_pick_kernel<T, VEC>, PICK_SMEM);
