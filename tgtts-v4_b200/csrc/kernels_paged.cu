@@ -183,20 +183,22 @@ TG_DEVICE void put4(bf16 *o, float4 v) {
     *reinterpret_cast<uint2 *>(o) =
         make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
 }
+// Two consecutive values, at an even place.
+template <typename C>
+TG_DEVICE float2 load2(const C *p);
+template <>
+TG_DEVICE float2 load2<float>(const float *p) { return __ldcs(reinterpret_cast<const float2 *>(p)); }
+template <>
+TG_DEVICE float2 load2<bf16>(const bf16 *p) {
+    const uint32_t r = __ldcs(reinterpret_cast<const uint32_t *>(p));
+    return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+}
+TG_DEVICE void put2(float *o, float2 v) { *reinterpret_cast<float2 *>(o) = v; }
+TG_DEVICE void put2(bf16 *o, float2 v) { *reinterpret_cast<__nv_bfloat162 *>(o) = __floats2bfloat162_rn(v.x, v.y); }
 TG_DEVICE void turn(float &a, float &b, float co, float si) {
     const float na = __fmaf_rn(a, co, -__fmul_rn(b, si));
     b = __fmaf_rn(b, co, __fmul_rn(a, si));
     a = na;
-}
-
-// Where a row's head is stored: null when the row does not write it.
-template <typename T>
-TG_DEVICE T *rope_out(const tg_params &p, const Divisor &page, uint32_t row, uint32_t head, uint32_t to, T *q, T *k, T *v) {
-    if (head < p.heads) return q + ((size_t)row * p.heads + head) * p.head_dim;
-    if (to == SPARE) return nullptr;
-    const bool value = head >= p.heads + p.kv_heads;
-    const uint32_t id = page.div(to), off = to - id * p.capacity, h = head - p.heads - (value ? p.kv_heads : 0);
-    return (value ? v : k) + (((size_t)id * p.kv_heads + h) * p.capacity + off) * p.head_dim;
 }
 
 // False for a row that writes nothing.
@@ -283,30 +285,75 @@ __global__ void __launch_bounds__(ROPE_THREADS)
     }
 }
 
-// Any other even rotated part: a pair to a thread (2047 rows of 48 heads of 128: 31 us, 9 where a thread takes eight).
+// Any other even rotated part, where fours of the two halves or of the tables' rows do not lie on 16 bytes: a thread takes
+// pair u of ROPE_PAIRS heads (apart by a ROPE_PAIRS-th of the heads), in the same order of rows. 2047 rows of 48 heads of 128, 100 turned:
+// 24 us (4 heads 24-27, 8 more), against 9 where a thread takes eight dimensions: the few bytes of a thread's loads in
+// flight bound it.
+constexpr int ROPE_PAIRS = 2;
+
 template <typename T, typename C>
 __global__ void __launch_bounds__(ROPE_THREADS)
-    rope_pages_any_kernel(tg_params p, Divisor page, Divisor row_units, uint32_t block_rows, const uint32_t *__restrict__ at,
-                          const uint32_t *__restrict__ place, const C *__restrict__ c, const float *__restrict__ cosv,
-                          const float *__restrict__ sinv, T *__restrict__ q, T *__restrict__ k, T *__restrict__ v, uint32_t *err) {
+    rope_pages_any_kernel(tg_params p, Divisor page, uint32_t units, uint32_t row_units, uint32_t block_rows,
+                          const uint32_t *__restrict__ at, const uint32_t *__restrict__ place, const C *__restrict__ c,
+                          const float *__restrict__ cosv, const float *__restrict__ sinv, T *__restrict__ q, T *__restrict__ k,
+                          T *__restrict__ v, uint32_t *err) {
+    const uint32_t hd = p.head_dim, heads = p.heads + 2 * p.kv_heads, apart = (heads + ROPE_PAIRS - 1) / ROPE_PAIRS, half = p.k / 2;
+    const uint32_t sub = threadIdx.x / units, unit = blockIdx.y * units + threadIdx.x % units;
+    const uint32_t head0 = unit / (hd / 2), u = unit % (hd / 2);
+    const bool rotated = p.rope && u < half;
+    // Of each head: where its first value lies in a row of c, where its pair's do in q's row or a page's position, and
+    // the pair: dimensions 2 u and 2 u + 1, or u and u + half of a head that turns in the half layout.
+    const C *x[ROPE_PAIRS];
+    T *o[ROPE_PAIRS];
+    bool here[ROPE_PAIRS], paged[ROPE_PAIRS], turned[ROPE_PAIRS], halves[ROPE_PAIRS];
+#pragma unroll
+    for (int n = 0; n < ROPE_PAIRS; n++) {
+        const uint32_t head = head0 + n * apart;
+        here[n] = unit < row_units && head < heads;
+        paged[n] = head >= p.heads;
+        turned[n] = rotated && head < p.heads + p.kv_heads;
+        halves[n] = turned[n] && !(p.flags & 1);
+        const uint32_t in = halves[n] ? u : 2 * u;
+        x[n] = c + (size_t)head * hd + in;
+        T *cache = head < p.heads + p.kv_heads ? k + (size_t)(head - p.heads) * p.capacity * hd
+                                               : v + (size_t)(head - p.heads - p.kv_heads) * p.capacity * hd;
+        o[n] = (paged[n] ? cache : q + (size_t)head * hd) + in;
+    }
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t units = p.head_dim / 2, heads = p.heads + 2 * p.kv_heads;
-    const uint32_t row0 = blockIdx.x * block_rows, here = min(block_rows, p.rows - row0) * row_units.d;
-    for (uint32_t i = threadIdx.x; i < here; i += ROPE_THREADS) {
-        const uint32_t in_block = row_units.div(i), row = row0 + in_block, in_row = i - in_block * row_units.d;
-        const uint32_t u = in_row % units, head = in_row / units, pos = at[row], to = place[row];
+    const size_t row_values = (size_t)heads * hd, row_q = (size_t)p.heads * hd, page_values = (size_t)p.kv_heads * p.capacity * hd;
+    const uint32_t step = gridDim.x * block_rows;
+    for (uint32_t row = blockIdx.x * block_rows + sub; row < p.rows; row += step) {
+        float a[ROPE_PAIRS], b[ROPE_PAIRS];
+#pragma unroll
+        for (int n = 0; n < ROPE_PAIRS; n++) {
+            if (!here[n]) continue;
+            const C *from = x[n] + row * row_values;
+            if (halves[n]) {
+                a[n] = to_f32<C>(from[0]);
+                b[n] = to_f32<C>(from[half]);
+            } else {
+                const float2 two = load2<C>(from);
+                a[n] = two.x;
+                b[n] = two.y;
+            }
+        }
+        const uint32_t pos = at[row], to = place[row];
         if (!rope_row(p, pos, to, err)) continue;
-        T *o = rope_out(p, page, row, head, to, q, k, v);
-        if (!o) continue;
-        const C *x = c + ((size_t)row * heads + head) * p.head_dim;
-        const bool turned = p.rope && head < p.heads + p.kv_heads && u < p.k / 2;
-        const bool half = turned && !(p.flags & 1);
-        const uint32_t d0 = half ? u : 2 * u, d1 = half ? p.k / 2 + u : 2 * u + 1;
-        float a = to_f32<C>(x[d0]), b = to_f32<C>(x[d1]);
-        if (turned) turn(a, b, __ldg(cosv + (size_t)pos * (p.k / 2) + u), __ldg(sinv + (size_t)pos * (p.k / 2) + u));
-        o[d0] = from_f32<T>(a);
-        o[d1] = from_f32<T>(b);
+        const float co = rotated ? __ldg(cosv + (size_t)pos * half + u) : 1.0f, si = rotated ? __ldg(sinv + (size_t)pos * half + u) : 0.0f;
+        const uint32_t id = page.div(to);
+        const size_t at_q = row * row_q, at_page = id * page_values + (size_t)(to - id * p.capacity) * hd;
+#pragma unroll
+        for (int n = 0; n < ROPE_PAIRS; n++) {
+            if (!here[n] || (paged[n] && to == SPARE)) continue;
+            T *out = o[n] + (paged[n] ? at_page : at_q);
+            if (turned[n]) turn(a[n], b[n], co, si);
+            if (halves[n]) {
+                out[0] = from_f32<T>(a[n]);
+                out[half] = from_f32<T>(b[n]);
+            } else
+                put2(out, make_float2(a[n], b[n]));
+        }
     }
 }
 
@@ -603,21 +650,18 @@ cudaError_t rope_t(const tg_params &p, const uint32_t *at, const uint32_t *place
                    const float *sn, void *q, void *k, void *v, uint32_t *err, cudaStream_t s) {
     const uint32_t heads = p.heads + 2 * p.kv_heads;
     const Divisor page(p.capacity);
-    if (p.k % 8) {
-        const uint32_t units = heads * (p.head_dim / 2), block_rows = units >= ROPE_THREADS ? 1 : ROPE_THREADS / units;
-        return launch_pdl(rope_pages_any_kernel<T, C>, dim3((p.rows + block_rows - 1) / block_rows), dim3(ROPE_THREADS), 0, s, p, page,
-                          Divisor(units), block_rows, at, place, (const C *)c, cs, sn, (T *)q, (T *)k, (T *)v, err);
-    }
     // A row's units over gridDim.y blocks of about equal width; as many rows to a block as fit; no more blocks than
     // four waves of four an SM (more rows to a thread then: 45.7 us for 32768 rows of 20 heads of 64; sixteen waves or a
     // thread a row 47.3 and 51.3, one wave 52.1).
-    const uint32_t row_units = (heads + 1) / 2 * (p.head_dim / 8), ny = (row_units + ROPE_THREADS - 1) / ROPE_THREADS;
+    const bool eights = p.k % 8 == 0;
+    const uint32_t row_units = eights ? (heads + 1) / 2 * (p.head_dim / 8) : (heads + ROPE_PAIRS - 1) / ROPE_PAIRS * (p.head_dim / 2), ny = (row_units + ROPE_THREADS - 1) / ROPE_THREADS;
     const uint32_t units = (row_units + ny - 1) / ny, block_rows = ROPE_THREADS / units;
     const uint32_t nx = min((p.rows + block_rows - 1) / block_rows, 4u * 4 * 148 / ny + 1);
     auto run = [&](auto kern) {
         return launch_pdl(kern, dim3(nx, ny), dim3(units * block_rows), 0, s, p, page, units, row_units, block_rows, at, place, (const C *)c, cs, sn,
                           (T *)q, (T *)k, (T *)v, err);
     };
+    if (!eights) return run(rope_pages_any_kernel<T, C>);
     if (p.head_dim == 64) return p.flags & 1 ? run(rope_pages_kernel<T, C, true, 64>) : run(rope_pages_kernel<T, C, false, 64>);
     return p.flags & 1 ? run(rope_pages_kernel<T, C, true, 128>) : run(rope_pages_kernel<T, C, false, 128>);
 }
