@@ -198,7 +198,9 @@ def rope_oracle(c64, cos, sin, at, place, old64, rot, inter, heads, kv, page, q6
     (37, 16, 2, 128, 128, False, 48, "bf16", "bf16"), (300, 20, 4, 128, 96, True, 64, "bf16", "bf16"),
     (5, 8, 8, 64, 2, False, 16, "f32", "f32"), (65, 8, 8, 64, 20, True, 128, "bf16", "f32"),
     (11, 4, 1, 64, 42, False, 16, "bf16", "bf16"), (70, 16, 2, 64, 8, False, 32, "f32", "f32"),
-    (19, 32, 8, 128, 0, False, 32, "bf16", "f32")])
+    (19, 32, 8, 128, 0, False, 32, "bf16", "f32"), (5000, 5, 1, 64, 50, False, 16, "bf16", "f32"),
+    (5000, 7, 7, 64, 30, True, 16, "f32", "f32"), (1200, 32, 8, 128, 100, True, 48, "bf16", "bf16"),
+    (1200, 20, 4, 128, 102, False, 32, "bf16", "f32")])
 def test_rope_pages(pkg, ctx, syn, rows, heads, kv, hd, rot, inter, page, dtype, ctype):
     pages, c, c64, cos, sin, at, place, old, old64 = rope_case(syn, rows, heads, kv, hd, rot, page, 500, dtype, ctype, rows + rot)
     if rows > 4:
