@@ -371,7 +371,8 @@ def batch(rng, rows, top, per=1):
     (1, 16, 2, 64, 32, 0, 1, 1), (1, 4, 1, 64, 16, 1, 1, 1), (3, 16, 2, 64, 48, 127, 40, 1), (2, 8, 8, 64, 16, 128, 300, 1),
     (9, 16, 2, 128, 32, 129, 17, 2), (17, 20, 4, 128, 64, 1000, 500, 3), (40, 16, 2, 64, 128, 2500, 700, 1),
     (33, 32, 8, 128, 16, 640, 130, 1), (70, 4, 1, 64, 16, 4097, 65, 5), (700, 32, 8, 128, 16, 130, 40, 1),
-    (300, 8, 8, 64, 32, 0, 400, 1), (1300, 16, 2, 64, 48, 40, 20, 4)])
+    (300, 8, 8, 64, 32, 0, 400, 1), (1300, 16, 2, 64, 48, 40, 20, 4), (40, 8, 8, 64, 32, 3001, 20, 1),
+    (5, 32, 8, 128, 16, 9000, 30, 1)])
 def test_attention_pages(pkg, ctx, syn, dtype, rows, heads, kv, hd, page, first, top, per):
     rng = np.random.default_rng(rows * 7 + first)
     lengths, of, back = batch(rng, rows, top, per)
