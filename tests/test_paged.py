@@ -117,3 +117,15 @@ def test_the_rest_of_the_table_tells_its_bindings_too(pkg, syn):
     p = pkg.params(shape, "bf16", rows=2, slots=2)
     assert pkg.needs("rmsnorm", p) == [2 * 1024 * 4, 1024 * 4, 2 * 1024 * 4]
     assert np.all(np.array(pkg.needs("rope_rows", p)) > 0)
+
+
+@pytest.mark.parametrize("count", [1, 2, 3])
+def test_arrays_of_few_entries_hold_those_alone(pkg, count):
+    """16 bytes stand in for an array without entries; one to three entries are four bytes each."""
+    assert pkg.needs("page_plan", plan(pkg, n=count))[2] == 4 * count
+    assert pkg.needs("attention_pages", heads(pkg, first=32 * count, seqs=5, stride=6))[5] == 4 * count
+    assert pkg.needs("rope_pages", heads(pkg, rope=1, k=2, n=count))[3:5] == [4 * count, 4 * count]
+    assert pkg.needs("logits_pick", pick(pkg, k=count))[1] == 4 * count
+    assert pkg.needs("logits_pick", pick(pkg, k1=count))[4:6] == [4 * count, 4 * count]
+    assert pkg.needs("logits_pick", pick(pkg, n=32 * count, m=1))[6] == 4 * count
+    assert pkg.needs("logits_pick", pick(pkg, n=30, m=count))[6] == 4 * count

@@ -735,3 +735,80 @@ def test_a_step_of_all_four_enqueued_and_captured_on_other_streams(pkg, ctx, syn
         for n in ("out", "q", "pick", "logits", "place"):
             m[n].fill(0)
     del graph
+
+
+# ---- arrays of one to three entries, bound as those alone ------------------------------------------------
+
+
+def exact(pkg, ctx, a, around=0x7FC00007):
+    """The array as a binding of its own bytes, in a buffer whose other words are not what a kernel may use."""
+    a = np.ascontiguousarray(a)
+    words = np.full(64, around, np.uint32)
+    words[4:4 + a.size] = a.reshape(-1).view(np.uint32)
+    return put(pkg, ctx, words), 16, a.nbytes
+
+
+def whole(m):
+    return m, 0, m.nbytes
+
+
+@pytest.mark.parametrize("count", [1, 2, 3])
+def test_short_arrays_page_plan(pkg, ctx, count):
+    held, fresh, free = np.zeros(4, np.uint32), np.full(4, 5, np.uint32), np.array([6, 2, 4], np.uint32)[:count]
+    table = np.full((4, 2), SPARE, np.uint32)
+    want, _ = plan_oracle(held, fresh, free, table, 20, 16, 8, 9)
+    p = pkg.TgParams(seqs=4, rows=20, stride=2, n=count, capacity=16, slots=8, first=9)
+    out = dict(table=put(pkg, ctx, table))
+    for name in ("at", "place", "starts", "next", "counts"):
+        out[name] = put(pkg, ctx, np.full(want[name].size, 0x77777777, np.uint32))
+    pkg.dispatch_once(ctx, "page_plan", p, [whole(put(pkg, ctx, held)), whole(put(pkg, ctx, fresh)), exact(pkg, ctx, free),
+                                            *map(whole, out.values())])
+    assert want["counts"][2] == count
+    for name in want:
+        assert np.array_equal(out[name].read(np.uint32, want[name].size), want[name].reshape(-1)), name
+
+
+@pytest.mark.parametrize("count", [1, 2, 3])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_short_arrays_rope_pages(pkg, ctx, syn, count, dtype):
+    rows, heads, kv, hd, page = 6, 4, 1, 64, 16
+    pages, c, c64, cos, sin, at, place, old, old64 = rope_case(syn, rows, heads, kv, hd, 2, page, count, dtype, "f32", count)
+    p = pkg.TgParams(dtype=pkg.DTYPES[dtype], heads=heads, kv_heads=kv, head_dim=hd, rows=rows, capacity=page, slots=pages, rope=1, k=2, n=count)
+    q0, q064 = typed(syn, np.zeros((rows, heads, hd)), dtype)
+    q, k, v = put(pkg, ctx, q0), put(pkg, ctx, old), put(pkg, ctx, old)
+    pkg.dispatch_once(ctx, "rope_pages", p, [*(whole(put(pkg, ctx, a)) for a in (at, place, c)), exact(pkg, ctx, cos), exact(pkg, ctx, sin),
+                                             whole(q), whole(k), whole(v)])
+    want = rope_oracle(c64, cos, sin, at, place, old64, 2, False, heads, kv, page, q064)
+    for got, w in zip((read(syn, q, dtype, q0.shape), read(syn, k, dtype, old.shape), read(syn, v, dtype, old.shape)), want):
+        # As test_rope_pages's.
+        assert np.all(np.abs(got - w) <= HALF_STEP[dtype] * np.abs(w) + 2 * 12 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("count", [1, 2, 3])
+@pytest.mark.parametrize("dtype", ["f32"])
+def test_short_arrays_attention_pages(pkg, ctx, syn, count, dtype):
+    b = Paged(syn, dtype, 16, 2, 64, 32, 32 * count, [5, 40], [0, 1], [0, 0], seed=count)
+    p = b.params(pkg)
+    out, work = put(pkg, ctx, np.zeros(b.q.shape, b.q.dtype)), pkg.Memory(ctx, pkg.attention_pages_work(p))
+    pkg.dispatch_once(ctx, "attention_pages", p, [*(whole(put(pkg, ctx, a)) for a in (b.q, b.k, b.v, b.at, b.table)), exact(pkg, ctx, b.shared),
+                                                  whole(work), whole(out)])
+    b.check(syn, out)
+
+
+@pytest.mark.parametrize("count", [1, 2, 3])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_short_arrays_logits_pick(pkg, ctx, syn, count, dtype):
+    rng = np.random.default_rng(count)
+    vocab = 32 * count
+    x, x64 = typed(syn, rng.standard_normal((2, vocab)), dtype)
+    seen, ids = np.array([7, 3, 7], np.uint32)[:count], np.array([30, 3, 9], np.uint32)[:count]
+    bias, bits = rng.standard_normal(count).astype(np.float32), rng.integers(0, 2 ** 32, (1, count), dtype=np.uint64).astype(np.uint32)
+    spans = np.array([[0, 1, count - 1, 0, count, 0], [0, 0, count, 0, 0, SPARE]], np.uint32)
+    pen = np.array([[1.5, 0.25, 0.5], [0.75, 1, 2]], np.float32)
+    p = pkg.TgParams(dtype=pkg.DTYPES[dtype], rows=2, n=vocab, stride=vocab, k=count, k1=count, m=1)
+    out, pick = put(pkg, ctx, np.zeros(x.shape, x.dtype)), put(pkg, ctx, np.zeros(2, np.uint32))
+    pkg.dispatch_once(ctx, "logits_pick", p, [whole(put(pkg, ctx, x)), exact(pkg, ctx, seen, 5), whole(put(pkg, ctx, spans)),
+                                              whole(put(pkg, ctx, pen)), exact(pkg, ctx, ids, 5), exact(pkg, ctx, bias), exact(pkg, ctx, bits),
+                                              whole(out), whole(pick)])
+    want, size = pick_oracle(x64, seen, spans, pen, ids, bias, bits, vocab)
+    pick_check(read(syn, out, dtype, x.shape), pick.read(np.uint32, 2), want, size, vocab, dtype, range(2))

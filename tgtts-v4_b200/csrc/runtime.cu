@@ -85,7 +85,8 @@ static int needs(const Launch &l, std::vector<Need> &out) {
     const uint64_t cache = slots * kvh * cap * hd * T;
     const uint64_t chunks = attn_chunks((uint32_t)cap);
     const uint64_t table = cap * (hd / 2) * F;
-    auto some = [](const char *name, uint64_t bytes) { return Need{name, std::max<uint64_t>(bytes, 16), bytes == 0}; };
+    // An array that may be empty: its own bytes, or any 16 where it has none.
+    auto some = [](const char *name, uint64_t bytes) { return Need{name, bytes ? bytes : 16, bytes == 0}; };
     switch (l.kernel) {
         case TG_KERNEL_RMSNORM:
             out = {{"x", rows * H * F}, {"gain", H * F}, {"out", rows * H * F}};
