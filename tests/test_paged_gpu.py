@@ -785,7 +785,7 @@ def test_short_arrays_rope_pages(pkg, ctx, syn, count, dtype):
 
 
 @pytest.mark.parametrize("count", [1, 2, 3])
-@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_short_arrays_attention_pages(pkg, ctx, syn, count, dtype):
     b = Paged(syn, dtype, 16, 2, 64, 32, 32 * count, [5, 40], [0, 1], [0, 0], seed=count)
     p = b.params(pkg)
@@ -812,3 +812,92 @@ def test_short_arrays_logits_pick(pkg, ctx, syn, count, dtype):
                                               whole(out), whole(pick)])
     want, size = pick_oracle(x64, seen, spans, pen, ids, bias, bits, vocab)
     pick_check(read(syn, out, dtype, x.shape), pick.read(np.uint32, 2), want, size, vocab, dtype, range(2))
+
+
+# ---- steps back to back, each from words that the one before stored ---------------------------------------
+
+
+class Steps:
+    """A run of serving steps whose words all come from the device: step i plans from the lengths that step i - 1 stored,
+    appends its rows' keys and values to pages it has just handed out, and attends to them behind a shared prefix. Only
+    the fresh counts, the free pages and the projections' outputs are given."""
+
+    def __init__(self, pkg, ctx, syn, dtype, hd, first, steps, seed=0):
+        rng = np.random.default_rng(seed)
+        self.pkg, self.ctx, self.steps = pkg, ctx, steps
+        heads, kv, page, seqs, rows, width, pages = 16, 2, 16, 48, 64, 24, 900
+        es = 2 if dtype == "bf16" else 4
+        order = rng.permutation(pages).astype(np.uint32)
+        shared, order = order[:max(4, -(-first // page))], order[max(4, -(-first // page)):]
+        held = rng.integers(0, 150, seqs).astype(np.uint32)
+        table = np.full((seqs, width), SPARE, np.uint32)
+        for s in range(seqs):
+            n = -(-int(held[s]) // page)
+            table[s, :n], order = order[:n], order[n:]
+        kv0 = [typed(syn, rng.standard_normal((pages, kv, page, hd)), dtype)[0] for _ in range(2)]
+        angle = np.arange(first + 400)[:, None] * 10000.0 ** (-2 * np.arange(hd // 2) / hd)
+        m = {"shared": shared, "k": kv0[0], "v": kv0[1], "cos": np.cos(angle).astype(np.float32), "sin": np.sin(angle).astype(np.float32),
+             "held0": held, "table": table}
+        self.start = {n: m[n] for n in ("k", "v", "held0", "table")}
+        for i in range(steps):
+            m[f"fresh{i}"] = rng.integers(0, 2, seqs).astype(np.uint32)
+            # As if held pages were many steps' apart: each step hands out pages of its own.
+            m[f"free{i}"], order = order[:seqs], order[int(seqs // 8):]
+            m[f"c{i}"] = rng.standard_normal((rows, (heads + 2 * kv) * hd)).astype(np.float32)
+        self.m = m = {n: put(pkg, ctx, a) for n, a in m.items()}
+        base = dict(dtype=pkg.DTYPES[dtype], heads=heads, kv_heads=kv, head_dim=hd, rows=rows, capacity=page, slots=pages, first=first,
+                    seqs=seqs, stride=width)
+        attend = pkg.TgParams(**base)
+        for n, size in (("at", 8 * rows), ("place", 4 * rows), ("starts", 4 * seqs + 4), ("held1", 4 * seqs), ("counts", 16),
+                        ("q", rows * heads * hd * es), ("work", pkg.attention_pages_work(attend))):
+            m[n] = pkg.Memory(ctx, size)
+        self.list = []
+        for i in range(steps):
+            m[f"out{i}"] = pkg.Memory(ctx, rows * heads * hd * es)
+            for kernel, p, names in (
+                    ("page_plan", pkg.TgParams(**{**base, "n": seqs}), f"held{i % 2} fresh{i} free{i} table at place starts held{1 - i % 2} counts"),
+                    ("rope_pages", pkg.TgParams(**{**base, "rope": 1, "k": hd, "n": first + 400}), f"at place c{i} cos sin q k v"),
+                    ("attention_pages", attend, f"q k v at table shared work out{i}")):
+                self.list.append((kernel, p, [whole(m[n]) for n in names.split()]))
+
+    def reset(self):
+        for n, a in self.start.items():
+            self.m[n].write(a)
+        for n in ("held1", "at", "place", "q", "work", *(f"out{i}" for i in range(self.steps))):
+            self.m[n].fill(0)
+        self.ctx.synchronize()
+
+    def results(self):
+        return {n: self.m[n].read(np.uint8, self.m[n].nbytes) for n in ("k", "v", "table", "held0", "held1", *(f"out{i}" for i in range(self.steps)))}
+
+
+@pytest.mark.parametrize("dtype,hd,first", [("bf16", 64, 700), ("bf16", 128, 1500), ("f32", 64, 300), ("bf16", 64, 0), ("bf16", 128, 1)])
+def test_steps_back_to_back_are_the_same_bits_as_steps_waited_for(pkg, ctx, syn, dtype, hd, first):
+    import torch
+
+    run_ = Steps(pkg, ctx, syn, dtype, hd, first, steps=8, seed=first)
+    run_.reset()
+    for kernel, p, bindings in run_.list:
+        pkg.dispatch_once(ctx, kernel, p, bindings)
+    want = run_.results()
+    counts = run_.m["counts"].read(np.uint32, 4)
+    assert counts[1] > 0 and counts[2] == 48  # rows were placed, and no request was left out
+    calls = [pkg.Dispatch(ctx, *step) for step in run_.list]
+    side = torch.cuda.Stream()
+
+    def enqueue(stream):
+        for d in calls:
+            d.enqueue(stream)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        enqueue(torch.cuda.current_stream().cuda_stream)
+    for go in (lambda: enqueue(side.cuda_stream), lambda: enqueue(0), graph.replay, graph.replay):
+        run_.reset()
+        go()
+        torch.cuda.synchronize()
+        ctx.synchronize()  # no error word
+        got = run_.results()
+        for n in want:
+            assert np.array_equal(got[n], want[n]), n
+    del graph

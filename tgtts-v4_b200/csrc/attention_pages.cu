@@ -233,8 +233,7 @@ TG_DEVICE uint64_t mn_desc(uint32_t addr, uint32_t chunk) {
 // pages by cp.async, OWN_STAGES - 1 chunks ahead of the products. e keeps 16 bits because a row's own positions are
 // few and may carry its whole sum; the second product costs nothing here, as the caches' bytes bound the
 // kernel: a head reads 4 hd bytes a position for 4 hd x group operations. What is needed is bytes in flight: 11
-// one-warp blocks an SM of two 8 KB stages each hold 90 KB of them, and, as small blocks, find room beside
-// prefix_kernel's (four warps to a block: 64 rows of 1024 behind 16384 positions 67 us against 55). 64 rows of up to 1024, 8 KV
+// one-warp blocks an SM of two 8 KB stages each hold 90 KB of them. 64 rows of up to 1024, 8 KV
 // heads of 128 (142 MB): 34 us with the join, 4.2 TB/s; 128 rows (268 MB) 56 us, 4.8 TB/s. Pieces of 128
 // positions, so that the longest row is no one warp's.
 constexpr int OWN_WARPS = 1, OWN_STAGES = 2;
@@ -262,10 +261,10 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
     extern __shared__ __align__(128) unsigned char own_mem[];
     __shared__ uint32_t total_s;
     constexpr int CH = own_chunk(HD), VECS = HD / 8, G16 = CH / 16, ROWS = 32 / VECS;
-    // Behind prefix_kernel this one starts under it: that kernel lets it go once what comes before both has
-    // ended (its own wait), and the two share nothing. One block waits for it all the same before it ends, so that
-    // the join waits for both; the others make room for the next.
-    if (np == 0) pdl_wait();
+    // Every block waits, behind prefix_kernel too: the rows' words, the table and the pages may be the stores of kernels
+    // before both, and this wait alone makes them visible here. (Under prefix_kernel, with a block's wait at its end, 64 rows
+    // behind 16384 positions took 55 us against 63, but nothing ordered its loads behind those stores.)
+    pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3, mi = lane >> 3, rr = lane & 7;
     const int heads = p.heads, kvh = p.kv_heads, group = heads / kvh;
@@ -470,7 +469,6 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
             }
         }
     }
-    if (blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 // ---- shared pieces, bf16 ------------------------------------------------------------------------------
@@ -491,7 +489,7 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
 //              its sum l is of the f32 values.
 // HD = 64: two tiles, which share the keys' copies, each with S, P and O in 256 columns. HD = 128: one tile
 // with two S buffers (S 2 x 128, P 64, O 128), as two tiles do not fit TMEM's 512 columns.
-// The softmax warps take registers from the first four (setmaxnreg), so that own_kernel's blocks find room beside.
+// The softmax warps take registers from the first four (setmaxnreg).
 // A tile of 128 keys takes about 2400 clocks (hd 64: 3400 for two tiles of queries), of which a softmax thread's
 // exponentials and sums are 1400, its waits and TMEM's loads and stores the rest; keys and values come
 // from L2 at up to 7.5 TB/s over all SMs meanwhile. No part bounds it alone: without the exponentials, or most of the
@@ -966,8 +964,8 @@ bool map_heads(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t outer,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Opts a kernel into its shared memory with all of an SM's as shared memory, so that blocks of the kernels that run
-// beside it find room there.
+// Opts a kernel into its shared memory with all of an SM's as shared memory, so that blocks of the next kernel, which
+// start under it and wait, find room there.
 template <typename F>
 cudaError_t with_all_smem(F kernel, size_t bytes) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
