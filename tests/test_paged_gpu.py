@@ -901,3 +901,106 @@ def test_steps_back_to_back_are_the_same_bits_as_steps_waited_for(pkg, ctx, syn,
         for n in want:
             assert np.array_equal(got[n], want[n]), n
     del graph
+
+
+# ---- calls of different sizes at the same time -------------------------------------------------------------
+
+
+def plan_call(pkg, ctx, seqs):
+    """A plan of one fresh position a request, as a call, with what it makes and how that is read."""
+    held, fresh, free, table, pages = plan_case(seqs, 16, 40, 1, seed=seqs)
+    fresh[:] = 1
+    old = -(-held.astype(np.int64) // 16)
+    new = -(-(held.astype(np.int64) + 1) // 16)
+    width = int(new.max())
+    table = np.full((seqs, width), SPARE, np.uint32)
+    ids = np.arange(int(new.sum()), dtype=np.uint32)
+    for s, at in enumerate(np.cumsum(old) - old):
+        table[s, :old[s]] = ids[at:at + old[s]]
+    free = ids[int(old.sum()):]
+    want, bad = plan_oracle(held, fresh, free, table, seqs, 16, len(ids), 3)
+    assert not bad
+    p = pkg.TgParams(seqs=seqs, rows=seqs, stride=width, n=len(free), capacity=16, slots=len(ids), first=3)
+    out = dict(table=put(pkg, ctx, table))
+    for name in ("at", "place", "starts", "next", "counts"):
+        out[name] = put(pkg, ctx, np.zeros(want[name].size, np.uint32))
+    call = pkg.Dispatch(ctx, "page_plan", p, [whole(put(pkg, ctx, a)) for a in (held, fresh, free)] + [whole(m) for m in out.values()])
+    return call, out, want
+
+
+def plan_call_check(out, want):
+    for name in want:
+        assert np.array_equal(out[name].read(np.uint32, want[name].size), want[name].reshape(-1)), name
+
+
+def linear_call(pkg, ctx, k):
+    """A projection of one row over k inputs, as a call; its shared memory grows with k."""
+    rng = np.random.default_rng(k)
+    x, w = rng.standard_normal(k).astype(np.float32), rng.standard_normal((8, k)).astype(np.float32)
+    out = dict(y=put(pkg, ctx, np.zeros(8, np.float32)))
+    mems = [put(pkg, ctx, a) for a in (x, x, w, np.zeros(8, np.float32))] + [out["y"]]
+    call = pkg.Dispatch(ctx, "gemv_linear", pkg.TgParams(dtype=pkg.F32, rows=1, slots=1, n=8, k=k, stride=8), [whole(m) for m in mems])
+    return call, out, (w.astype(np.float64) @ x, np.abs(w.astype(np.float64)) @ np.abs(x), k)
+
+
+def linear_call_check(out, want):
+    y, size, k = want
+    # A sum of k products in f32.
+    assert np.all(np.abs(out["y"].read(np.float32, 8) - y) <= (k + 1) * 2.0 ** -24 * size)
+
+
+@pytest.mark.parametrize("make,check,sizes", [(plan_call, plan_call_check, (16384, 3000)), (plan_call, plan_call_check, (5000, 16384, 4000, 9)),
+                                              (linear_call, linear_call_check, (6000, 2000, 1200, 4096))])
+def test_calls_of_different_sizes_enqueued_from_several_threads(pkg, ctx, make, check, sizes):
+    import threading
+
+    import torch
+
+    made = [make(pkg, ctx, n) for n in sizes]
+    ctx.synchronize()
+    streams, failed = [torch.cuda.Stream() for _ in sizes], []
+    start = threading.Barrier(len(sizes))
+
+    def work(call, stream):
+        start.wait()
+        for i in range(1500):
+            try:
+                call.enqueue(stream.cuda_stream)
+            except pkg.Error as e:
+                failed.append(f"{i}: {e}")
+                return
+            if i % 100 == 99:
+                stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(made[i][0], streams[i])) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    assert not failed, failed
+    for _, out, want in made:
+        check(out, want)
+
+
+def test_a_captured_call_replays_after_smaller_and_larger_ones(pkg, ctx):
+    import torch
+
+    big, out, want = plan_call(pkg, ctx, 12000)
+    others = [plan_call(pkg, ctx, n) for n in (4000, 16384, 8)]
+    ctx.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        big.enqueue(torch.cuda.current_stream().cuda_stream)
+    for other, *_ in others:
+        out["place"].fill(0)
+        out["at"].fill(0)
+        other.enqueue(ctx.stream)
+        ctx.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        plan_call_check(out, want)
+    for _, o, w in others:
+        plan_call_check(o, w)
+    del graph

@@ -1454,7 +1454,7 @@ size_t decode_step_flag_bytes(int layers) {
 template <typename T, int NB>
 static cudaError_t launch_step_t(const PersistArgs &a, int sms, size_t smem, size_t flag_bytes, cudaStream_t s) {
     auto kern = decode_step_kernel<T, NB>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = with_smem(kern, smem);
     if (e != cudaSuccess) return e;
     int per_sm = 0;
     if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, PS_THREADS, smem)) != cudaSuccess) return e;

@@ -463,7 +463,7 @@ cudaError_t launch_dtc(DtcArgs a, const void *w, int tiles, const DtcPlan &pl, c
     a.cc = pl.cc;
     a.a_bytes = pl.a_bytes;
     auto kern = dtc_kernel<EPI>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem);
+    cudaError_t e = with_smem(kern, pl.smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(pl.S, tiles, 1);

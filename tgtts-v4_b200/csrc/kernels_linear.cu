@@ -85,9 +85,8 @@ cudaError_t launch_gemv_linear(const tg_params &p, const float *x0, const float 
     const size_t smem = (size_t)LIN_NB * K * sizeof(float);
     const dim3 grid((p.n + LIN_WARPS - 1) / LIN_WARPS);
     auto go = [&](auto kern, const auto *wt) {
-        cudaError_t e = cudaSuccess;
-        if (smem > 32 * 1024 && (e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)))
-            return e;
+        const cudaError_t e = with_smem(kern, smem);
+        if (e != cudaSuccess) return e;
         kern<<<grid, LIN_WARPS * 32, smem, s>>>(p, x0, x1, wt, bias, out);
         return cudaGetLastError();
     };

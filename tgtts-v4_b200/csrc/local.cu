@@ -430,7 +430,7 @@ cudaError_t launch_proj(const void *x, const void *w, int M, int N, int K, int p
     LocalProjArgs a{static_cast<const uint8_t *>(w), M, N, K, K / parts, K / LP_BK, pl.NT, pl.nkb, pl.kb_stage,
                     pl.stages, pl.w_stage, pl.stage_bytes, pl.tmem_cols, partial, out, err};
     auto kern = local_proj_kernel<EPI>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem);
+    cudaError_t e = with_smem(kern, pl.smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(kern, dim3(N / 128, parts, pl.chunks), dim3(LP_THREADS), pl.smem, s, xm, a);
 }

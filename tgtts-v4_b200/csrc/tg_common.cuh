@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "tgcuda.h"
 
 #define TG_DEVICE __device__ __forceinline__
@@ -310,13 +312,19 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// Opts a kernel into a launch's dynamic shared memory. The limit is one for all of a device's launches of the kernel,
+// so it is only ever raised: another thread may be about to launch with more.
 template <typename F>
 inline cudaError_t with_smem(F kernel, size_t bytes) {
     // Past 48 KiB of shared memory a block needs the opt-in, static arrays included: opt in well
     // before.
     if (bytes <= 32 * 1024) return cudaSuccess;
+    static std::mutex mu;  // between the look and the change
+    const std::lock_guard<std::mutex> lock(mu);
+    cudaFuncAttributes now;
+    const cudaError_t e = cudaFuncGetAttributes(&now, kernel);
+    if (e != cudaSuccess || (size_t)now.maxDynamicSharedSizeBytes >= bytes) return e;
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
-
 
 }  // namespace tg
