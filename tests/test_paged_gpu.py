@@ -1004,3 +1004,134 @@ def test_a_captured_call_replays_after_smaller_and_larger_ones(pkg, ctx):
     for _, o, w in others:
         plan_call_check(o, w)
     del graph
+
+
+# ---- one key among thousands --------------------------------------------------------------------------------
+
+
+NEEDLE = 1.0 + np.arange(128) * 5 % 16  # the values at a needle, other ones at its neighbours
+
+
+def needles(syn, b, spots, strength=20.0):
+    """Row r's queries all point along dimension r % len(spots), as the key at spots[r % len(spots)] alone does (a position
+    of the prefix, or from `first` on the row's own): the row's output is that position's values, up to e^-20 or so."""
+    rng = np.random.default_rng(1)
+    k, v, q = b.k64.copy(), b.v64.copy(), np.zeros_like(b.q64)
+    for r in range(b.rows):
+        j = r % len(spots)
+        q[r] = 0.05 * rng.standard_normal(q[r].shape)
+        q[r, :, j] = strength
+        if b.at[r] == SPARE:
+            continue
+        t, s = spots[j], int(b.at[b.rows + r])
+        pg = b.shared[t // b.page] if t < b.first else b.table[s, (t - b.first) // b.page]
+        off = (t if t < b.first else t - b.first) % b.page
+        k[pg, :, off] = 0.0
+        k[pg, :, off, j] = strength
+        v[pg, :, off] = NEEDLE[j]
+    (b.k, b.k64), (b.v, b.v64), (b.q, b.q64) = (typed(syn, a, b.dtype) for a in (k, v, q))
+
+
+def edges(steps, end):
+    """Positions beside multiples of the steps, the first and the last, below `end`."""
+    out = {0, end - 1}
+    for s in steps:
+        for t in range(s, end + 1, s):
+            out |= {t - 1, t}
+    return sorted(t for t in out if t < end)
+
+
+@pytest.mark.parametrize("dtype,heads,kv,hd,page,first", [
+    ("bf16", 16, 2, 64, 16, 1000), ("bf16", 16, 2, 64, 64, 8191), ("bf16", 32, 8, 128, 16, 1500), ("bf16", 8, 4, 128, 48, 6001),
+    ("bf16", 4, 1, 128, 128, 2049), ("bf16", 20, 4, 64, 32, 4100), ("bf16", 12, 4, 128, 32, 700), ("f32", 16, 2, 64, 32, 1000),
+    ("f32", 8, 8, 128, 16, 400)])
+def test_attention_pages_finds_one_key_of_the_prefix(pkg, ctx, syn, dtype, heads, kv, hd, page, first):
+    """Keys beside the edges of pages, of copies' boxes, of tiles and of pieces, in the first and second half of a tile;
+    the queries of a tile move their references at different tiles."""
+    spots = edges((128, page), first) + [t + 64 for t in edges((128,), first - 64)] + [t + 16 for t in edges((128,), first - 16)]
+    spots = [int(spots[i]) for i in np.linspace(0, len(spots) - 1, min(len(spots), hd)).astype(int)]
+    spots = sorted(set(spots) | {0, first - 1})[:hd]
+    spots[-1] = first - 1
+    rows = 2 * len(spots) + 3
+    b = Paged(syn, dtype, heads, kv, hd, page, first, [3] * rows, list(range(rows)), [0] * rows, seed=first)
+    needles(syn, b, spots)
+    out = b.run(pkg, ctx)
+    b.check(syn, out)
+    got = read(syn, out, dtype, b.q.shape)
+    assert np.all(np.abs(got - NEEDLE[np.arange(rows) % len(spots)][:, None, None]) < 0.5)
+
+
+@pytest.mark.parametrize("dtype,heads,kv,hd,page,first", [
+    ("bf16", 16, 2, 64, 16, 0), ("bf16", 32, 8, 128, 16, 0), ("bf16", 16, 2, 128, 48, 300), ("bf16", 5, 1, 64, 128, 77),
+    ("f32", 16, 2, 64, 32, 0), ("f32", 4, 1, 128, 16, 30)])
+def test_attention_pages_finds_one_key_of_its_own(pkg, ctx, syn, dtype, heads, kv, hd, page, first):
+    """Keys beside the edges of pages, chunks and pieces of a request's own positions."""
+    spots = [first + t for t in edges((16, 128), 395)]
+    spots = [spots[i] for i in np.linspace(0, len(spots) - 1, min(len(spots), hd)).astype(int)]
+    rows = len(spots)
+    b = Paged(syn, dtype, heads, kv, hd, page, first, [395] * rows, list(range(rows)), [0] * rows, seed=page)
+    needles(syn, b, spots)
+    out = b.run(pkg, ctx)
+    b.check(syn, out)
+    got = read(syn, out, dtype, b.q.shape)
+    assert np.all(np.abs(got - NEEDLE[:rows][:, None, None]) < 0.5)
+
+
+@pytest.mark.parametrize("hd,first", [(64, 3000), (128, 1500), (128, 5000)])
+@pytest.mark.parametrize("scale", [8.0, 30.0])
+def test_attention_pages_with_peaked_scores_over_several_tiles_of_queries(pkg, ctx, syn, hd, first, scale):
+    rows = 70
+    lengths = [int(n) for n in np.random.default_rng(hd).integers(1, 500, rows)]
+    b = Paged(syn, "bf16", 16, 2, hd, 32, first, lengths, list(range(rows)), [0] * rows, seed=hd, scale=scale)
+    b.check(syn, b.run(pkg, ctx))
+
+
+# ---- large vocabularies and long histories -------------------------------------------------------------------
+
+
+def wide_case(syn, rows, vocab, stride, hist, dtype, seed, flat=False):
+    """Rows over a large vocabulary with histories of as many different tokens as `hist` even draws give. `flat`: whole
+    logits with many equal largest ones and controls that change nothing."""
+    rng = np.random.default_rng(seed)
+    base = rng.integers(-3, 3, stride) if flat else 4 * rng.standard_normal(stride)
+    x = np.stack([np.roll(base, 977 * r) for r in range(rows)])
+    if flat:
+        for r in range(rows):  # equal largest values beside the ends of runs, tiles and blocks' shares
+            t = np.concatenate([rng.integers(0, vocab, 4)] + [np.arange(e - 2, e + 2) for e in range(4096, vocab, 4096 * (1 + r % 5))])
+            x[r, rng.choice(t[t < vocab], min(6, len(t)), replace=False)] = 5
+    x, x64 = typed(syn, x, dtype)
+    seen = rng.integers(0, vocab, max(1, hist)).astype(np.uint32)
+    spans = np.zeros((rows, 6), np.uint32)
+    spans[:, 5] = SPARE
+    if hist:
+        spans[:, 0] = rng.integers(0, hist // 8, rows)
+        spans[:, 1] = hist // 4
+        spans[:, 2] = hist - hist // 4 - spans[:, 0]
+    if not flat:
+        spans[::3, 5] = 0
+    pen = np.tile(np.array([[1, 0, 0]], np.float32), (rows, 1)) if flat else np.stack(
+        [rng.uniform(0.8, 2, rows), rng.uniform(-1, 1, rows), rng.uniform(-1, 1, rows)], 1).astype(np.float32)
+    ids, bias = rng.integers(0, vocab, 40).astype(np.uint32), (3 * rng.standard_normal(40)).astype(np.float32)
+    if not flat:
+        spans[1::2, 4] = 40
+    bits = rng.integers(0, 2 ** 32, (1, (vocab + 31) // 32), dtype=np.uint64).astype(np.uint32)
+    return x, x64, seen, spans, pen, ids, bias, bits
+
+
+@pytest.mark.parametrize("rows,vocab,stride,hist,dtype,in_place,flat", [
+    # Two runs of a block's bit map (past 65,536 of its tokens): without controls, with them, with ties, odd ends.
+    (66, 150001, 150016, 0, "f32", False, False), (66, 150001, 150016, 0, "bf16", True, True), (66, 150001, 150008, 500, "f32", True, False),
+    (66, 150001, 150016, 500, "bf16", False, False), (66, 150001, 150001, 400, "bf16", True, False), (66, 140001, 140004, 300, "f32", False, True),
+    (3, 530003, 530003, 900, "f32", False, False),
+    # More than 4096, and than 8192, different touched tokens in a block's share: runs cut shorter.
+    (2, 131000, 131072, 60000, "f32", False, False), (2, 131000, 131072, 60000, "bf16", True, True), (66, 40001, 40008, 60000, "bf16", False, False),
+    (66, 40001, 40004, 60000, "f32", True, True), (1, 20000, 20000, 200000, "f32", False, True), (66, 150001, 150004, 90000, "f32", False, False)])
+def test_logits_pick_over_several_runs(pkg, ctx, syn, rows, vocab, stride, hist, dtype, in_place, flat):
+    x, x64, seen, spans, pen, ids, bias, bits = wide_case(syn, rows, vocab, stride, hist, dtype, rows + vocab, flat)
+    out, pick, bad = pick_run(pkg, ctx, x, seen, spans, pen, ids, bias, bits, vocab, 1, dtype, in_place)
+    assert not bad
+    got = read(syn, out, dtype, x.shape)
+    want, size = pick_oracle(x64, seen, spans, pen, ids, bias, bits, vocab)
+    pick_check(got, pick, want, size, vocab, dtype, range(rows))
+    left = x64[:, vocab:] if in_place else np.full((rows, stride - vocab), 12.0625 if dtype == "bf16" else 7.0)
+    assert np.array_equal(got[:, vocab:], left)
