@@ -236,8 +236,9 @@ typedef enum {
      * (i, i + k / 2), or (2 i, 2 i + 1) with params.flags bit 0, the others as they are; all as they
      * are when params.rope is 0 (k 0, cos and sin any 16 bytes). A row whose position is TG_SPARE
      * writes nothing; one whose place is TG_SPARE writes q alone. A position of n or more, or a
-     * place past the cache, is skipped with the kernel error word. Of rows with the same place one,
-     * not said which, is kept. */
+     * place past the cache, is skipped with the kernel error word. The places of a
+     * dispatch's rows are distinct: where two rows have the same one, each value stored there is one of theirs, not
+     * said whose, so that the position may hold a mixture of both. */
     TG_KERNEL_ROPE_PAGES = 28,
     /* q T [rows][heads][hd], k pages T, v pages T, at u32 [2 rows] (a position of at least `first`,
      * then a request), table u32 [seqs][stride], shared u32 [ceil(first / capacity)] (any 16 bytes

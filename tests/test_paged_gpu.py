@@ -245,6 +245,37 @@ def test_rope_pages_is_rope_rows_over_slots(pkg, ctx, syn, dtype):
         assert np.array_equal(a.read(np.uint8, a.nbytes), b.read(np.uint8, b.nbytes))
 
 
+@pytest.mark.parametrize("hd,rot,dtype", [(64, 64, "bf16"), (128, 96, "f32"), (64, 42, "bf16")])
+def test_rope_pages_rows_with_one_place_leave_values_of_theirs(pkg, ctx, syn, hd, rot, dtype):
+    """Every value at a place that several rows have is one of these rows' (of any of them: the position may be a
+    mixture); the rows' queries and the other places are as ever."""
+    rows, heads, kv, page = 600, 16, 2, 32
+    pages, c, c64, cos, sin, at, place, old, old64 = rope_case(syn, rows, heads, kv, hd, rot, page, 50, dtype, "f32", rot)
+    place[1::3] = place[0::3]
+    place[500:520] = place[40]
+    p = pkg.TgParams(dtype=pkg.DTYPES[dtype], heads=heads, kv_heads=kv, head_dim=hd, rows=rows, capacity=page, slots=pages, rope=1, k=rot, n=50)
+    q0, q064 = typed(syn, np.zeros((rows, heads, hd)), dtype)
+    q, k, v = put(pkg, ctx, q0), put(pkg, ctx, old), put(pkg, ctx, old)
+    run(pkg, ctx, "rope_pages", p, [put(pkg, ctx, a) for a in (at, place, c, cos, sin)] + [q, k, v])
+    got_k, got_v = (read(syn, m, dtype, old.shape) for m in (k, v))
+    fits = {}
+    got_q = read(syn, q, dtype, q0.shape)
+    for r in range(rows):  # a row at a time, so that each of a place's rows is compared with what is there
+        wq, wk, wv = rope_oracle(c64[r:r + 1], cos, sin, at[r:r + 1], place[r:r + 1], old64, rot, False, heads, kv, page, q064[r:r + 1])
+        t = int(place[r])
+        for n, (got, w) in enumerate(((got_k, wk), (got_v, wv))):
+            g, w = got[t // page, :, t % page], w[t // page, :, t % page]
+            near = np.abs(g - w) <= HALF_STEP[dtype] * np.abs(w) + 2 * 12 * 2.0 ** -24  # as test_rope_pages's
+            fits[t, n] = fits.get((t, n), False) | near
+        assert np.all(np.abs(got_q[r] - wq[0]) <= HALF_STEP[dtype] * np.abs(wq[0]) + 2 * 12 * 2.0 ** -24)
+    assert all(f.all() for f in fits.values())
+    free = np.ones(pages * page, bool)
+    free[place] = False
+    for got in (got_k, got_v):
+        flat = lambda a: a.transpose(0, 2, 1, 3).reshape(pages * page, -1)[free]  # noqa: E731
+        assert np.array_equal(flat(got), flat(old64))
+
+
 def test_rope_pages_skips_words_that_point_outside(pkg, ctx, syn):
     rows, heads, kv, hd, page = 9, 4, 1, 64, 16
     pages, c, c64, cos, sin, at, place, old, old64 = rope_case(syn, rows, heads, kv, hd, hd, page, 40, "f32", "f32", 2)
