@@ -246,7 +246,10 @@ typedef enum {
      * contents free between dispatches, so dispatches in one stream may share it)
      * -> out T [rows][heads][hd]: each row attends to the shared prefix and to its request's own
      * positions up to its own, softmax(q k / sqrt(hd)) v. The prefix is read once for many rows.
-     * Rows may belong to one request (several new positions, each seeing those before it). A spare
+     * For bf16 products are summed
+     * in f32; the weights e^(s - m) of own positions enter the second product as two bf16 (16 bits), those of the shared
+     * prefix as one, so that an output is off by up to 2^-8 of its values' weighted sizes there before its own rounding;
+     * their sum is f32. Rows may belong to one request (several new positions, each seeing those before it). A spare
      * row's output is left. A position below `first` or past the table, a request of seqs or more,
      * or a page past the cache is reported by the kernel error word (the row's output is left, or
      * for a page meaningless). A row's result is the same bits whatever rows run beside it, for one
@@ -315,7 +318,7 @@ int tg_dispatch_once(tg_ctx *ctx, const tg_dispatch *d, double *ns);
 /* A dispatch for callers with streams of their own: resolved and checked once, as a program's, then
  * enqueued as often as needed on any stream of the context's device (a cudaStream_t; NULL: the legacy
  * stream; TG_ECUDA for another device's), without waiting. An enqueue allocates nothing and may be
- * captured into the caller's CUDA graph. The buffers have to live until the work is done; what the
+ * captured into the caller's CUDA graph. The context and the buffers have to live until the work is done; what the
  * kernels report in the context's error word comes with the next tg_ctx_synchronize after that. One
  * call may be enqueued from several threads, or on several streams, where the work itself may overlap. */
 typedef struct tg_call tg_call;

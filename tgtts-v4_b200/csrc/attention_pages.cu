@@ -25,9 +25,10 @@ constexpr uint32_t OWN_PIECE = 128;
 // n / d, rounded up.
 __host__ __device__ inline uint32_t shares(uint32_t n, uint32_t d) { return n / d + (n % d != 0); }
 // Shared positions of a piece, whole tiles of 128: at most 16 pieces; 8 while those are at most 512 and at most 64 x KV
-// heads long, as the KV heads make units too. (Behind 4096 positions, 8 KV heads of 128, pieces of 512 against 256: 32 rows
-// 19.6 us against 24.7, 128 rows 75 against 84, one row 13.7 against 12.1. Behind 16384 pieces of 2048 against 1024: 64 rows
-// 53 against 55, one row 29 against 20.)
+// heads long, as the KV heads make units too. (Rows of one own position behind 4096, 8 KV heads of 128,
+// pieces of 512 against 256: one row 17.3 us against 17.0, 32 rows 20.3 against 20.5, 64 rows 23.0 against 26.7, 128 rows
+// 34 against 41. Behind 16384 pieces of 2048 against 1024: one row 33 against 25, 32 rows 36 against 29, 64 rows 39 against
+// 42, 128 rows 64 against 70. Behind 8191, 2 KV heads of 64, pieces of 1024 against 512: 128 rows 31 against 24.)
 __host__ __device__ inline uint32_t shared_piece(const tg_params &p) {
     const uint32_t most = p.kv_heads < 8 ? 64 * p.kv_heads : 512, even = shares(p.first, 8);
     const uint32_t longer = even < most ? even : most, size = longer > shares(p.first, 16) ? longer : shares(p.first, 16);
@@ -69,7 +70,7 @@ TG_DEVICE bool paged_row(const tg_params &p, const uint32_t *at, int row, uint32
 // Products, sums and statistics in f32; the references are natural.
 // Bound by the shared memory reads that feed the multiply-adds (three of 16 bytes to 32 of those). One launch for
 // both kinds of piece: two cost 5 us more in a call of 10 rows. 32 queries a block against one row's heads:
-// 128 rows of 16 heads over 2 at head dim 64 behind 4096 shared positions in 119 us against 211, 18 TFLOP/s.
+// 128 rows of 16 heads over 2 at head dim 64 behind 4096 shared positions in 118 us against 211, 18 TFLOP/s.
 constexpr int F32_THREADS = 256, F32_QUERIES = 32;
 template <int HD, int QN>
 struct F32 {
@@ -234,7 +235,8 @@ TG_DEVICE uint64_t mn_desc(uint32_t addr, uint32_t chunk) {
 // few and may carry its whole sum; the second product costs nothing here, as the caches' bytes bound the
 // kernel: a head reads 4 hd bytes a position for 4 hd x group operations. What is needed is bytes in flight: 11
 // one-warp blocks an SM of two 8 KB stages each hold 90 KB of them. 64 rows of up to 1024, 8 KV
-// heads of 128 (142 MB): 34 us with the join, 4.2 TB/s; 128 rows (268 MB) 56 us, 4.8 TB/s. Pieces of 128
+// heads of 128 (143 MB, not in L2): 34.8 us with the join, 4.1 TB/s; 128 rows (268 MB) 62 us, 4.3 TB/s (four warps to a
+// block: 36.3 and 59 us; 64 rows behind 16384 shared positions 70 with one, 72 with four). Pieces of 128
 // positions, so that the longest row is no one warp's.
 constexpr int OWN_WARPS = 1, OWN_STAGES = 2;
 constexpr int own_chunk(int hd) { return 2048 / hd; }
@@ -262,8 +264,8 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
     __shared__ uint32_t total_s;
     constexpr int CH = own_chunk(HD), VECS = HD / 8, G16 = CH / 16, ROWS = 32 / VECS;
     // Every block waits, behind prefix_kernel too: the rows' words, the table and the pages may be the stores of kernels
-    // before both, and this wait alone makes them visible here. (Under prefix_kernel, with a block's wait at its end, 64 rows
-    // behind 16384 positions took 55 us against 63, but nothing ordered its loads behind those stores.)
+    // before both, and this wait alone makes them visible here. (Run under prefix_kernel without it, 64 rows behind 1024 positions
+    // took 13 us against 22, 64 behind 16384 55 against 70, but nothing ordered the loads behind those stores.)
     pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3, mi = lane >> 3, rr = lane & 7;
@@ -491,10 +493,11 @@ __global__ void __launch_bounds__(OWN_WARPS * 32)
 // with two S buffers (S 2 x 128, P 64, O 128), as two tiles do not fit TMEM's 512 columns.
 // The softmax warps take registers from the first four (setmaxnreg).
 // A tile of 128 keys takes about 2400 clocks (hd 64: 3400 for two tiles of queries), of which a softmax thread's
-// exponentials and sums are 1400, its waits and TMEM's loads and stores the rest; keys and values come
-// from L2 at up to 7.5 TB/s over all SMs meanwhile. No part bounds it alone: without the exponentials, or most of the
-// products, or with P in two places, the time is the same within 3%. Storing a unit's partials takes 5000 clocks.
-// Alone: 128 rows of 16 heads over 2 of 64 behind 8191 positions 15.5 us, 64 rows of 32 over 8 of 128 behind 16384 33 us.
+// exponentials and sums are 1400, its waits and TMEM's loads and stores the rest. No unit is near its rate: hd 128 (hd 64)
+// has the tensor cores busy 22% (11%) of the time, the exponentials' pipe 31% (34%), L2 at 21% (7%) and
+// HBM at 25% (3%) of theirs. The chain of S, softmax, P and PV with its waits bounds a tile. Storing a unit's partials
+// takes 5000 clocks. Alone, from cold caches: 128 rows of 16 heads over 2 of 64 behind 8191 positions 18.1 us, 64 rows
+// of 32 over 8 of 128 behind 16384 35.6 us (256 units over 148 SMs: two rounds, the second for 108).
 // Every wait is bounded (the context's error word, then the block runs out).
 template <int HD>
 struct Pfx {
@@ -881,7 +884,7 @@ __global__ void __launch_bounds__(Pfx<HD>::THREADS) __maxnreg__(Pfx<HD>::REGS)
 // Joins the partials of a row's head, a block to it: 16 bytes of a piece's o to a lane, the pieces over the
 // block's groups of HD / 4 lanes, all loads of a row of up to JOIN_DEEP pieces a group in flight at once; the
 // groups' sums are then added in order. References are in base 2 for bf16, natural for f32. Latency-bound, then by
-// the partials' bytes from L2: 2048 heads of 16 + 2 pieces of 64 5 us, of 16 + 5 pieces of 128 9 us.
+// the partials' bytes: from cold caches 2048 heads of 16 + up to 6 pieces of 64 (10 MB) 10.2 us, of 16 + up to 8 of 128 (22 MB) 11.2.
 constexpr int JOIN_THREADS = 128, JOIN_DEEP = 8;
 
 template <typename T, int HD>

@@ -34,8 +34,8 @@ struct Divisor {
 // the requests' words; a row finds its request by bisection of the sums. All requests up to the first
 // one that does not fit are served, so the sums over served requests are the sums over all.
 // Latency-bound: a load of the requests' words (all in flight at once), the scan, the bisection and a row's load of
-// its page's number follow one another. 2048 requests with 82,000 rows: 7.3 us of a run of launches (twice as many
-// blocks 8.7, a quarter 9.0: they read the same words); 8 requests 3.1, about an empty launch.
+// its page's number follow one another. 2048 requests with 82,000 rows: 7.4 us of a run of launches (twice as many
+// blocks 8.5, a quarter 9.5: they read the same words); 8 requests 3.0, about an empty launch.
 constexpr int PLAN_THREADS = 512;
 constexpr int PLAN_ROWS = 1024;  // rows a block, up to PLAN_BLOCKS blocks
 constexpr uint32_t PLAN_BLOCKS = 148;
@@ -215,7 +215,7 @@ TG_DEVICE bool rope_row(const tg_params &p, uint32_t pos, uint32_t to, uint32_t 
 // which turn by the same angles), rotated ones as four pairs (in the half layout two runs of four, each a warp's
 // whole sectors), of every gridDim-th group of rows: where they lie in a row is worked out once. All of a
 // row's loads of c leave before it is known whether the row is spare. 32768 rows of 20 heads of 64, f32 to bf16 (253
-// MB): 45.7 us, 5.5 TB/s; 2047 rows of 48 heads of 128 (50 MB): 10.3 us.
+// MB): 46.4 us, 5.4 TB/s; 2047 rows of 48 heads of 128 (50 MB, not in L2): 13.9 us, 3.7 TB/s.
 constexpr int ROPE_THREADS = 256;
 
 template <typename T, typename C, bool INTER, int HD>
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(ROPE_THREADS)
 
 // Any other even rotated part, where fours of the two halves or of the tables' rows do not lie on 16 bytes: a thread takes
 // pair u of ROPE_PAIRS heads (apart by a ROPE_PAIRS-th of the heads), in the same order of rows. 2047 rows of 48 heads of 128, 100 turned:
-// 24 us (4 heads 24-27, 8 more), against 9 where a thread takes eight dimensions: the few bytes of a thread's loads in
+// 33 us (4 heads 37, 8 45), against 14 where a thread takes eight dimensions: the few bytes of a thread's loads in
 // flight bound it.
 constexpr int ROPE_PAIRS = 2;
 
@@ -366,9 +366,11 @@ __global__ void __launch_bounds__(ROPE_THREADS)
 // or eight to a 16-byte load and store (one by one in rows that 16 bytes do not divide); the touched ones' values
 // overwrite what the stream left. The row's greedy choice is joined over the cluster in distributed shared memory.
 // HBM-bound where there are rows enough: each logit is read and written once. 128 rows of 128,000 tokens in f32
-// (131 MB): 24.2 us without controls, 5.4 TB/s; 33 us with histories of 4096 tokens and 64 biases, whose two passes
-// come before the stream (under them the logits come into L2). One row of 32,000 with a history of 700: 6.8 us, the
-// passes' latencies. Counting inside the stream, a table of counts to a tile: 71 us for the 128 rows.
+// (131 MB, not in L2): 28.3 us without controls, 4.6 TB/s; 38.5 us with histories of 4096 tokens and 64 biases, whose two
+// passes come before the stream (under them the logits come into L2). One row of 32,000 with a history of 700: 6.2 us,
+// the passes' latencies. Counting inside the stream, a table of counts to a tile, took twice the time for the 128 rows.
+// A run in which more than PICK_TOUCHED different tokens are touched is cut to that many tokens, and the history is read
+// again for each: 64 rows with histories to 20,000 52.5 us, to 4000 20.1.
 constexpr int PICK_THREADS = 512;
 constexpr uint32_t PICK_TILE = 1024, PICK_AHEAD = 64 * PICK_TILE;
 constexpr uint32_t PICK_RUN = 65536;     // the most tokens whose bits are held at once
@@ -622,8 +624,8 @@ cudaError_t pick_t(const tg_params &p, const void *logits, const uint32_t *seen,
                    const uint32_t *ids, const float *bias, const uint32_t *masks, void *out, uint32_t *pick, uint32_t *err,
                    cudaStream_t s) {
     // Blocks of 1024 tokens at least; the most to a row that run at once (two an SM), up to eight. Of 128,000 tokens
-    // with 8, 4 and 2 blocks a row: 1 row 9.1, 12.2, 18.1 us; 32 rows 14.5, 18.3, 24.0; 64 rows 27.5, 20.7, 30.5; 128
-    // rows 54, 39, 34.
+    // with 8, 4 and 2 blocks a row: 1 row 6.8, 8.9, 13.0 us; 32 rows 10.8, 13.2, 18.5; 64 rows 20.3, 16.8, 21.9; 128
+    // rows 39, 31, 28 (without controls; with histories to 4096 55, 42, 39).
     uint32_t ranks = p.rows <= 32 ? 8 : p.rows <= 64 ? 4 : 2;
     while (ranks > 1 && p.n <= ranks / 2 * PICK_TILE) ranks /= 2;
     cudaError_t e = with_smem(logits_pick_kernel<T, VEC>, PICK_SMEM);
@@ -651,8 +653,8 @@ cudaError_t rope_t(const tg_params &p, const uint32_t *at, const uint32_t *place
     const uint32_t heads = p.heads + 2 * p.kv_heads;
     const Divisor page(p.capacity);
     // A row's units over gridDim.y blocks of about equal width; as many rows to a block as fit; no more blocks than
-    // four waves of four an SM (more rows to a thread then: 45.7 us for 32768 rows of 20 heads of 64; sixteen waves or a
-    // thread a row 47.3 and 51.3, one wave 52.1).
+    // four waves of four an SM (more rows to a thread then: 46.5 us for 32768 rows of 20 heads of 64; sixteen waves or a
+    // thread a row 50.2 and 51.5, one wave 57.9).
     const bool eights = p.k % 8 == 0;
     const uint32_t row_units = eights ? (heads + 1) / 2 * (p.head_dim / 8) : (heads + ROPE_PAIRS - 1) / ROPE_PAIRS * (p.head_dim / 2), ny = (row_units + ROPE_THREADS - 1) / ROPE_THREADS;
     const uint32_t units = (row_units + ny - 1) / ny, block_rows = ROPE_THREADS / units;
